@@ -33,11 +33,18 @@ SOURCES = [
     ('conv_grad.hip', []),
     ('bn_train.hip', []),
     ('gru_train.hip', []),
+    ('layer_norm.hip', []),
+    ('dropout.hip', []),
+    ('dropout_norm.hip', []),
     ('labels.hip', []),
     ('images.hip', []),
 ]
 # FIERY_CONV_TUNING=1: also build the convolution's clock-probe / priority variants (tools/microbench.py conv --clk)
 TUNING = ['-DFIERY_CONV_TUNING=1'] if os.environ.get('FIERY_CONV_TUNING') == '1' else ['-DFIERY_CONV_TUNING=0']
+# hipcc turns plain float code into packed fp32 instructions by itself; these translation units are built without them (a device
+# feature: hipcc's host pass warns that it does not know it)
+NO_PACKED_FP32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
+HIP_ONLY = {name: NO_PACKED_FP32 for name in ('layer_norm.hip', 'dropout.hip', 'dropout_norm.hip')}
 COMMON = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-I' + INCLUDE, '-I' + CSRC, '-x', 'hip']
 
 
@@ -59,14 +66,15 @@ def build(force=False, verbose=True):
         OUT = os.path.join(os.path.dirname(HERE), 'tools', 'ab', f'libfiery_hip_{variant}.so')
     os.makedirs(objdir, exist_ok=True)
     headers = [os.path.join(CSRC, 'common.h'), os.path.join(CSRC, 'conv_igemm_kernel.h'),
-               os.path.join(CSRC, 'fiery_gfx950.h'), os.path.join(INCLUDE, 'fiery_hip.h')]
+               os.path.join(CSRC, 'fiery_gfx950.h'), os.path.join(CSRC, 'fiery_row_types.h'), os.path.join(CSRC, 'row_ops.h'),
+               os.path.join(CSRC, 'layer_norm_kernel.h'), os.path.join(INCLUDE, 'fiery_hip.h')]
     objs, jobs = [], []
     for name, extra in SOURCES:
         src = os.path.join(CSRC, name)
         obj = os.path.join(objdir, name + '.o')
         objs.append(obj)
         if force or _stale(obj, [src] + headers):
-            cmd = [HIPCC] + COMMON + TUNING + os.environ.get('FIERY_BUILD_FLAGS', '').split() + extra + ['-c', src, '-o', obj]
+            cmd = [HIPCC] + COMMON + TUNING + os.environ.get('FIERY_BUILD_FLAGS', '').split() + extra + HIP_ONLY.get(name, []) + ['-c', src, '-o', obj]
             if verbose:
                 print(' '.join(cmd), flush=True)
             jobs.append((name, subprocess.Popen(cmd)))       # translation units compile side by side

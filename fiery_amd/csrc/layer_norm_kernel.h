@@ -1,0 +1,545 @@
+// Layer norm over the channels of pixel-major rows, forward and backward, alone or behind residual + dropout (JOIN).
+//
+//   h = x                                    (alone)         h = residual + drop(x)          (JOIN; mask: row_ops.h)
+//   mean = sum h / C,  var = sum (h - mean)^2 / C,  rstd = 1 / sqrt(var + eps),  xhat = (h - mean) rstd,  y = xhat gamma + beta
+//   backward:  gg = dy gamma,  dh' = [dh +] rstd (gg - (sum gg + xhat sum gg xhat) / C),
+//              dx = dh' (alone) or drop(dh'), dresidual = dh' (JOIN);  dgamma = sum over rows of dy xhat,  dbeta = sum dy.
+//
+// Memory-bound: every tensor is read once and written once.  A row lives in registers between its load and its store, so the
+// two sums (mean, then squared distances from it: no cancellation) cost no second pass.  A row is dealt to lanes in units of
+// eight columns (row_ops.h): a power-of-two group of up to 64 lanes of one wavefront (C <= 1024, no barrier), a workgroup (up
+// to 32768 forward, 16384 backward), or, past that, a workgroup that walks the row three times.
+// The backward pass deals a lane the same columns for all its rows, so dgamma and dbeta grow in registers; every workgroup
+// leaves one partial row and k_norm_finish adds them in a fixed order in double.  Sums and statistics are fp32; what is
+// stored in 16 bits is rounded once, at the store.
+// With a 16-bit stream y comes from the h before its rounding, while the statistics that are kept are those of the h that is
+// stored, which is what the backward pass reads: its xhat then sums to zero and has its variance, and the gradient is the norm's
+// at that h.  (With the other statistics a row of small variance beside a large mean had an xhat off by |mean| rstd / 256.)
+#pragma once
+#include "row_ops.h"
+
+namespace fiery {
+
+struct NormFwdArgs {
+    const void* x;
+    const void* residual;
+    const void* gamma;
+    const void* beta;
+    void* y;
+    void* h;
+    float* mean;                         // [rows], may be null (no backward pass will follow)
+    float* rstd;
+    long long x_ld, res_ld, y_ld, h_ld;
+    int rows, C, lane_bits, param_type;
+    float eps, inv_c;
+    DropArgs drop;
+};
+
+struct NormBwdArgs {
+    const void* dy;
+    const void* dh;                      // JOIN: gradient of h itself, may be null
+    const void* h;                       // the rows that were normalised (alone: x)
+    const void* gamma;
+    const float* mean;
+    const float* rstd;
+    void* dx;                            // may be null
+    void* dres;                          // JOIN, may be null
+    float* partial;                      // [workgroups][2][round_up(C, 8)]: dgamma, dbeta of a workgroup's rows; null: not wanted
+    void* dgamma;                        // written here by a single workgroup
+    void* dbeta;
+    long long dy_ld, dh_ld, h_ld, dx_ld, dres_ld;
+    int rows, C, lane_bits, param_type;
+    float inv_c;
+    DropArgs drop;
+};
+
+namespace {
+
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+    for (int m = 1; m < lanes; m <<= 1) v += __shfl_xor(v, m);
+    return v;
+}
+
+// Sum over the lanes that share a row, the same in all of them.  BLOCK: over the workgroup, through one of two slots used in
+// turn (a slot is written again only behind the barrier of the call in between).
+template <bool BLOCK, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], int lanes, float (*slots)[16][2], int& turn) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = lanes_sum(v[i], BLOCK ? 64 : lanes);
+    if constexpr (BLOCK) {
+        const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+        if ((threadIdx.x & 63) == 0)
+            for (int i = 0; i < N; ++i) slots[turn][wave][i] = v[i];
+        __syncthreads();
+        for (int i = 0; i < N; ++i) {
+            float s = 0.f;
+            for (int w = 0; w < waves; ++w) s += slots[turn][w][i];
+            v[i] = s;
+        }
+        turn ^= 1;
+    }
+}
+
+// s / C by the reciprocal and one correction: exact where the quotient is (the mean of a constant row is its value)
+__device__ __forceinline__ float mean_of(float s, int C, float inv_c) {
+    const float m = s * inv_c;
+    return fmaf(fmaf(-m, static_cast<float>(C), s), inv_c, m);
+}
+
+__device__ __forceinline__ int unit_count(int C, int unit) {
+    const int left = C - unit * kUnit;
+    return left >= kUnit ? kUnit : left > 0 ? left : 0;
+}
+
+// one unit of h: x alone, or residual + drop(x), written out as it is read
+template <typename T, typename S, bool JOIN>
+__device__ __forceinline__ void load_h(const NormFwdArgs& a, const DropKey& key, long long row, int unit, int count, bool write, float (&v)[kUnit]) {
+    const long long c = static_cast<long long>(unit) * kUnit;
+    load_unit<T>(static_cast<const typename T::store*>(a.x) + row * a.x_ld + c, count, v);
+    if constexpr (JOIN) {
+        float r[kUnit];
+        load_unit<S>(static_cast<const typename S::store*>(a.residual) + row * a.res_ld + c, count, r);
+        drop_unit(a.drop, key, static_cast<unsigned>(row), static_cast<unsigned>(unit), v);
+#pragma unroll
+        for (int j = 0; j < kUnit; ++j) v[j] += r[j];
+        if (write) store_unit<S>(static_cast<typename S::store*>(a.h) + row * a.h_ld + c, count, v);
+    }
+}
+
+template <typename S>
+__device__ __forceinline__ void sum_stored(const float (&v)[kUnit], float& s) {
+    float r[kUnit];
+    as_stored<S>(v, r);
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j) s += r[j];
+}
+template <typename S>
+__device__ __forceinline__ void distances_stored(const float (&v)[kUnit], int count, float mean, float& q) {
+    float r[kUnit];
+    as_stored<S>(v, r);
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j) {
+        const float d = j < count ? r[j] - mean : 0.f;
+        q += d * d;
+    }
+}
+
+template <typename T, typename S, bool JOIN, int NV, bool BLOCK>
+__global__ __launch_bounds__(BLOCK ? 1024 : 256) void k_norm_fwd(NormFwdArgs a) {
+    __shared__ float slots[2][16][2];
+    int turn = 0;
+    const int lanes = BLOCK ? static_cast<int>(blockDim.x) : 1 << a.lane_bits;
+    const int sub = static_cast<int>(threadIdx.x) & (lanes - 1);
+    const int per_block = BLOCK ? 1 : 256 >> a.lane_bits;
+    const int mine = BLOCK ? 0 : static_cast<int>(threadIdx.x) >> a.lane_bits;
+    DropKey key = {0, 0, 0, 0};
+    if constexpr (JOIN) {
+        if (a.drop.threshold) key = drop_key(a.drop);
+        drop_note(a.drop);
+    }
+    float ga[NV][kUnit], be[NV][kUnit];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < kUnit; ++j) {
+            const int c = (i * lanes + sub) * kUnit + j;
+            ga[i][j] = a.gamma && c < a.C ? load_typed(a.gamma, a.param_type, c) : 1.f;
+            be[i][j] = a.beta && c < a.C ? load_typed(a.beta, a.param_type, c) : 0.f;
+        }
+    // (every lane of a wavefront walks the loop as often as its neighbours: the exchanges need all of them)
+    for (long long first = static_cast<long long>(blockIdx.x) * per_block; first < a.rows; first += static_cast<long long>(gridDim.x) * per_block) {
+        const long long row = first + mine;
+        const bool live = row < a.rows;
+        constexpr bool two = JOIN && sizeof(typename S::store) == 2;            // the stored h has statistics of its own
+        float v[NV][kUnit];
+        int count[NV];
+        float s[two ? 2 : 1] = {}, q[two ? 2 : 1] = {};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int unit = i * lanes + sub;
+            count[i] = live ? unit_count(a.C, unit) : 0;
+            if constexpr (JOIN) {
+                for (int j = 0; j < kUnit; ++j) v[i][j] = 0.f;
+                if (count[i]) load_h<T, S, true>(a, key, row, unit, count[i], true, v[i]);
+            } else {
+                load_h<T, S, false>(a, key, live ? row : 0, unit, count[i], false, v[i]);
+            }
+#pragma unroll
+            for (int j = 0; j < kUnit; ++j) s[0] += v[i][j];
+            if constexpr (two) sum_stored<S>(v[i], s[1]);
+        }
+        row_sums<BLOCK>(s, lanes, slots, turn);
+        const float mean = mean_of(s[0], a.C, a.inv_c);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int j = 0; j < kUnit; ++j) {
+                const float d = j < count[i] ? v[i][j] - mean : 0.f;
+                q[0] += d * d;
+            }
+            if constexpr (two) distances_stored<S>(v[i], count[i], mean_of(s[1], a.C, a.inv_c), q[1]);
+        }
+        row_sums<BLOCK>(q, lanes, slots, turn);
+        const float rstd = 1.f / sqrtf(q[0] * a.inv_c + a.eps);
+        if (a.mean && live && sub == 0) {
+            a.mean[row] = two ? mean_of(s[two ? 1 : 0], a.C, a.inv_c) : mean;
+            a.rstd[row] = two ? 1.f / sqrtf(q[two ? 1 : 0] * a.inv_c + a.eps) : rstd;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float out[kUnit];
+#pragma unroll
+            for (int j = 0; j < kUnit; ++j) out[j] = (v[i][j] - mean) * rstd * ga[i][j] + be[i][j];
+            store_unit<T>(static_cast<typename T::store*>(a.y) + (live ? row : 0) * a.y_ld + static_cast<long long>(i * lanes + sub) * kUnit, count[i], out);
+        }
+    }
+}
+
+// Rows past what the registers of a workgroup hold: three walks over the row (sum, squared distances, result); the second and
+// third come out of the caches.
+template <typename T, typename S, bool JOIN>
+__global__ __launch_bounds__(1024) void k_norm_fwd_long(NormFwdArgs a) {
+    __shared__ float slots[2][16][2];
+    int turn = 0;
+    const int units = (a.C + kUnit - 1) / kUnit;
+    DropKey key = {0, 0, 0, 0};
+    if constexpr (JOIN) {
+        if (a.drop.threshold) key = drop_key(a.drop);
+        drop_note(a.drop);
+    }
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        constexpr bool two = JOIN && sizeof(typename S::store) == 2;
+        float v[kUnit], s[two ? 2 : 1] = {}, q[two ? 2 : 1] = {};
+        for (int u = threadIdx.x; u < units; u += blockDim.x) {
+            load_h<T, S, JOIN>(a, key, row, u, unit_count(a.C, u), true, v);
+#pragma unroll
+            for (int j = 0; j < kUnit; ++j) s[0] += v[j];
+            if constexpr (two) sum_stored<S>(v, s[1]);
+        }
+        row_sums<true>(s, 64, slots, turn);
+        const float mean = mean_of(s[0], a.C, a.inv_c);
+        for (int u = threadIdx.x; u < units; u += blockDim.x) {
+            const int count = unit_count(a.C, u);
+            load_h<T, S, JOIN>(a, key, row, u, count, false, v);
+#pragma unroll
+            for (int j = 0; j < kUnit; ++j) {
+                const float d = j < count ? v[j] - mean : 0.f;
+                q[0] += d * d;
+            }
+            if constexpr (two) distances_stored<S>(v, count, mean_of(s[1], a.C, a.inv_c), q[1]);
+        }
+        row_sums<true>(q, 64, slots, turn);
+        const float rstd = 1.f / sqrtf(q[0] * a.inv_c + a.eps);
+        if (a.mean && threadIdx.x == 0) {
+            a.mean[row] = two ? mean_of(s[two ? 1 : 0], a.C, a.inv_c) : mean;
+            a.rstd[row] = two ? 1.f / sqrtf(q[two ? 1 : 0] * a.inv_c + a.eps) : rstd;
+        }
+        for (int u = threadIdx.x; u < units; u += blockDim.x) {
+            const int count = unit_count(a.C, u);
+            load_h<T, S, JOIN>(a, key, row, u, count, false, v);
+#pragma unroll
+            for (int j = 0; j < kUnit; ++j)
+                if (j < count) {
+                    const long long c = static_cast<long long>(u) * kUnit + j;
+                    v[j] = (v[j] - mean) * rstd * (a.gamma ? load_typed(a.gamma, a.param_type, c) : 1.f) + (a.beta ? load_typed(a.beta, a.param_type, c) : 0.f);
+                }
+            store_unit<T>(static_cast<typename T::store*>(a.y) + row * a.y_ld + static_cast<long long>(u) * kUnit, count, v);
+        }
+    }
+}
+
+// One unit of the backward pass's results from its dy (gg = dy gamma), xhat and the row's sums.
+template <typename T, typename S, bool JOIN>
+__device__ __forceinline__ void store_grads(const NormBwdArgs& a, const DropKey& key, long long row, int unit, int count, const float (&gg)[kUnit],
+                                            const float (&xhat)[kUnit], float rstd, float m1, float m2) {
+    const long long c = static_cast<long long>(unit) * kUnit;
+    float out[kUnit];
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j) out[j] = rstd * (gg[j] - (m1 + xhat[j] * m2));
+    if constexpr (JOIN) {
+        if (a.dh) {
+            float d[kUnit];
+            load_unit<S>(static_cast<const typename S::store*>(a.dh) + row * a.dh_ld + c, count, d);
+#pragma unroll
+            for (int j = 0; j < kUnit; ++j) out[j] += d[j];
+        }
+        if (a.dres) store_unit<S>(static_cast<typename S::store*>(a.dres) + row * a.dres_ld + c, count, out);
+        if (!a.dx) return;
+        drop_unit(a.drop, key, static_cast<unsigned>(row), static_cast<unsigned>(unit), out);
+    } else {
+        if (!a.dx) return;
+    }
+    store_unit<T>(static_cast<typename T::store*>(a.dx) + row * a.dx_ld + c, count, out);
+}
+
+template <typename T, typename S, bool JOIN, int NV, bool BLOCK>
+__global__ __launch_bounds__(BLOCK ? 1024 : 256) void k_norm_bwd(NormBwdArgs a) {
+    typedef typename std::conditional<JOIN, S, T>::type H;
+    __shared__ float slots[2][16][2];
+    int turn = 0;
+    const int lanes = BLOCK ? static_cast<int>(blockDim.x) : 1 << a.lane_bits;
+    const int sub = static_cast<int>(threadIdx.x) & (lanes - 1);
+    const int per_block = BLOCK ? 1 : 256 >> a.lane_bits;
+    const int mine = BLOCK ? 0 : static_cast<int>(threadIdx.x) >> a.lane_bits;
+    DropKey key = {0, 0, 0, 0};
+    if constexpr (JOIN)
+        if (a.drop.threshold) key = drop_key(a.drop);
+    float ga[NV][kUnit], dg[NV][kUnit], db[NV][kUnit];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < kUnit; ++j) {
+            const int c = (i * lanes + sub) * kUnit + j;
+            ga[i][j] = a.gamma && c < a.C ? load_typed(a.gamma, a.param_type, c) : 1.f;
+            dg[i][j] = 0.f;
+            db[i][j] = 0.f;
+        }
+    for (long long first = static_cast<long long>(blockIdx.x) * per_block; first < a.rows; first += static_cast<long long>(gridDim.x) * per_block) {
+        const long long row = first + mine;
+        const bool live = row < a.rows;
+        const long long at = live ? row : 0;
+        const float mean = a.mean[at], rstd = a.rstd[at];
+        float gg[NV][kUnit], xhat[NV][kUnit], s[2] = {0.f, 0.f};
+        int count[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int unit = i * lanes + sub;
+            const long long c = static_cast<long long>(unit) * kUnit;
+            count[i] = live ? unit_count(a.C, unit) : 0;
+            load_unit<H>(static_cast<const typename H::store*>(a.h) + at * a.h_ld + c, count[i], xhat[i]);
+            load_unit<T>(static_cast<const typename T::store*>(a.dy) + at * a.dy_ld + c, count[i], gg[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < kUnit; ++j) {
+                xhat[i][j] = j < count[i] ? (xhat[i][j] - mean) * rstd : 0.f;
+                dg[i][j] += gg[i][j] * xhat[i][j];
+                db[i][j] += gg[i][j];
+                gg[i][j] *= ga[i][j];
+                s[0] += gg[i][j];
+                s[1] += gg[i][j] * xhat[i][j];
+            }
+        row_sums<BLOCK>(s, lanes, slots, turn);
+        const float m1 = s[0] * a.inv_c, m2 = s[1] * a.inv_c;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (count[i]) store_grads<T, S, JOIN>(a, key, at, i * lanes + sub, count[i], gg[i], xhat[i], rstd, m1, m2);
+    }
+    if (!a.partial && !a.dgamma && !a.dbeta) return;
+    const int width = (a.C + kUnit - 1) / kUnit * kUnit;
+    bool writes = true;
+    if constexpr (!BLOCK) {
+        // the lanes that hold the same columns: those of this wavefront, then the other three wavefronts', in order
+        __shared__ float others[3][NV * 64 * kUnit][2];
+        const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < kUnit; ++j) {
+                for (int m = lanes; m < 64; m <<= 1) {
+                    dg[i][j] += __shfl_xor(dg[i][j], m);
+                    db[i][j] += __shfl_xor(db[i][j], m);
+                }
+                if (wave > 0 && lane < lanes) {
+                    const int c = (i * lanes + lane) * kUnit + j;
+                    others[wave - 1][c][0] = dg[i][j];
+                    others[wave - 1][c][1] = db[i][j];
+                }
+            }
+        __syncthreads();
+        writes = wave == 0 && lane < lanes;
+        if (writes) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < kUnit; ++j)
+                    for (int w = 0; w < 3; ++w) {
+                        const int c = (i * lanes + lane) * kUnit + j;
+                        dg[i][j] += others[w][c][0];
+                        db[i][j] += others[w][c][1];
+                    }
+        }
+    }
+    if (!writes) return;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * lanes + sub) * kUnit;
+        if (c >= a.C) continue;
+        if (gridDim.x > 1) {
+            float* row = a.partial + static_cast<long long>(blockIdx.x) * 2 * width + c;
+            store_n<F32, 8>(row, dg[i]);
+            store_n<F32, 8>(row + width, db[i]);
+            continue;
+        }
+        for (int j = 0; j < kUnit && c + j < a.C; ++j) {
+            if (a.dgamma) store_typed(a.dgamma, a.param_type, c + j, dg[i][j]);
+            if (a.dbeta) store_typed(a.dbeta, a.param_type, c + j, db[i][j]);
+        }
+    }
+}
+
+// Rows past the registers: the row's sums in one walk, its results in a second; dgamma and dbeta in k_norm_bwd_cols_long.
+template <typename T, typename S, bool JOIN>
+__global__ __launch_bounds__(1024) void k_norm_bwd_long(NormBwdArgs a) {
+    typedef typename std::conditional<JOIN, S, T>::type H;
+    __shared__ float slots[2][16][2];
+    int turn = 0;
+    const int units = (a.C + kUnit - 1) / kUnit;
+    DropKey key = {0, 0, 0, 0};
+    if constexpr (JOIN)
+        if (a.drop.threshold) key = drop_key(a.drop);
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float gg[kUnit], xhat[kUnit], s[2] = {0.f, 0.f};
+        for (int walk = 0; walk < 2; ++walk) {
+            const float m1 = s[0] * a.inv_c, m2 = s[1] * a.inv_c;
+            for (int u = threadIdx.x; u < units; u += blockDim.x) {
+                const int count = unit_count(a.C, u);
+                const long long c = static_cast<long long>(u) * kUnit;
+                load_unit<H>(static_cast<const typename H::store*>(a.h) + row * a.h_ld + c, count, xhat);
+                load_unit<T>(static_cast<const typename T::store*>(a.dy) + row * a.dy_ld + c, count, gg);
+#pragma unroll
+                for (int j = 0; j < kUnit; ++j) {
+                    xhat[j] = j < count ? (xhat[j] - mean) * rstd : 0.f;
+                    if (a.gamma && j < count) gg[j] *= load_typed(a.gamma, a.param_type, c + j);
+                }
+                if (walk == 0) {
+#pragma unroll
+                    for (int j = 0; j < kUnit; ++j) {
+                        s[0] += gg[j];
+                        s[1] += gg[j] * xhat[j];
+                    }
+                } else {
+                    store_grads<T, S, JOIN>(a, key, row, u, count, gg, xhat, rstd, m1, m2);
+                }
+            }
+            if (walk == 0) row_sums<true>(s, 64, slots, turn);
+        }
+    }
+}
+
+// dgamma, dbeta of one unit of columns over the strip blockIdx.y of the rows, one partial row per strip
+template <typename T, typename H>
+__global__ __launch_bounds__(256) void k_norm_bwd_cols_long(NormBwdArgs a) {
+    const int unit = blockIdx.x * 256 + threadIdx.x, count = unit_count(a.C, unit);
+    if (count == 0) return;
+    const int width = (a.C + kUnit - 1) / kUnit * kUnit;
+    const long long c = static_cast<long long>(unit) * kUnit;
+    float dg[kUnit] = {}, db[kUnit] = {}, h[kUnit], g[kUnit];
+    for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        load_unit<H>(static_cast<const typename H::store*>(a.h) + row * a.h_ld + c, count, h);
+        load_unit<T>(static_cast<const typename T::store*>(a.dy) + row * a.dy_ld + c, count, g);
+        const float mean = a.mean[row], rstd = a.rstd[row];
+#pragma unroll
+        for (int j = 0; j < kUnit; ++j) {
+            dg[j] += j < count ? g[j] * ((h[j] - mean) * rstd) : 0.f;
+            db[j] += g[j];
+        }
+    }
+    float* out = a.partial + static_cast<long long>(blockIdx.y) * 2 * width + c;
+    store_n<F32, 8>(out, dg);
+    store_n<F32, 8>(out + width, db);
+}
+
+}  // namespace
+
+// ---- host side ---------------------------------------------------------------------------------------------------------------
+inline int row_ops_cus() {
+    static const int n_cu = [] {
+        int dev = 0, n = 0;
+        if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+        return n;
+    }();
+    return n_cu;
+}
+
+// How a row's units are dealt: NV units per lane, `threads` per workgroup, block = the workgroup shares the row; NV 0: long rows.
+struct NormShape {
+    int nv, threads, lane_bits;
+    bool block;
+    int per_block;                       // rows of one pass of a workgroup
+};
+inline NormShape norm_shape(int C, bool backward) {
+    const int units = (C + kUnit - 1) / kUnit;
+    if (units <= 128) {
+        int bits = 0;
+        while (bits < 6 && (1 << bits) < units) ++bits;
+        return {units <= 64 ? 1 : 2, 256, bits, false, 256 >> bits};
+    }
+    // 128 registers per lane at 1024 threads: forward holds 3 x 8 values a unit at most, backward 5 x 8
+    const int most = backward ? 2 : 4;
+    for (int nv = 1; nv <= most; nv *= 2)
+        for (int threads = 256; threads <= 1024; threads *= 2)
+            if (units <= nv * threads && (nv == most || threads <= 256 * nv)) return {nv, threads, 0, true, 1};
+    return {0, 1024, 0, true, 1};
+}
+// workgroups of the backward pass = partial rows of dgamma / dbeta
+inline int norm_bwd_blocks(int64_t rows, int C) {
+    const NormShape s = norm_shape(C, true);
+    if (s.nv == 0) return static_cast<int>(rows < 16 ? rows : 16);
+    const int64_t passes = (rows + s.per_block - 1) / s.per_block;
+    if (passes <= 2) return 1;
+    const int64_t most = static_cast<int64_t>(row_ops_cus()) * (s.block ? 1024 / s.threads : 4);
+    return static_cast<int>(passes < most ? passes : most);
+}
+inline int64_t norm_bwd_workspace_floats(int64_t rows, int C) {
+    return static_cast<int64_t>(norm_bwd_blocks(rows, C)) * 2 * ((C + kUnit - 1) / kUnit * kUnit);
+}
+
+void norm_finish(const NormBwdArgs& a, int blocks, hipStream_t stream);          // layer_norm.hip
+
+namespace {
+
+template <typename T, typename S, bool JOIN>
+void norm_fwd_launch(NormFwdArgs a, hipStream_t stream) {
+    const NormShape s = norm_shape(a.C, false);
+    a.lane_bits = s.lane_bits;
+    const long long passes = (static_cast<long long>(a.rows) + s.per_block - 1) / s.per_block;
+    const long long most = static_cast<long long>(row_ops_cus()) * (s.block ? 16384 / s.threads : 64);
+    const dim3 grid(static_cast<unsigned>(passes < most ? passes : most)), block(s.threads);
+    if (s.nv == 0)
+        hipLaunchKernelGGL((k_norm_fwd_long<T, S, JOIN>), grid, block, 0, stream, a);
+    else if (!s.block && s.nv == 1)
+        hipLaunchKernelGGL((k_norm_fwd<T, S, JOIN, 1, false>), grid, block, 0, stream, a);
+    else if (!s.block)
+        hipLaunchKernelGGL((k_norm_fwd<T, S, JOIN, 2, false>), grid, block, 0, stream, a);
+    else if (s.nv == 1)
+        hipLaunchKernelGGL((k_norm_fwd<T, S, JOIN, 1, true>), grid, block, 0, stream, a);
+    else if (s.nv == 2)
+        hipLaunchKernelGGL((k_norm_fwd<T, S, JOIN, 2, true>), grid, block, 0, stream, a);
+    else
+        hipLaunchKernelGGL((k_norm_fwd<T, S, JOIN, 4, true>), grid, block, 0, stream, a);
+}
+
+template <typename T, typename S, bool JOIN>
+void norm_bwd_launch(NormBwdArgs a, hipStream_t stream) {
+    typedef typename std::conditional<JOIN, S, T>::type H;
+    const NormShape s = norm_shape(a.C, true);
+    a.lane_bits = s.lane_bits;
+    const bool sums = a.dgamma || a.dbeta;
+    const int blocks = norm_bwd_blocks(a.rows, a.C);
+    if (!sums) a.partial = nullptr;
+    const dim3 grid(blocks), block(s.threads);
+    if (s.nv == 0) {
+        const int units = (a.C + kUnit - 1) / kUnit, most = 2 * row_ops_cus();
+        hipLaunchKernelGGL((k_norm_bwd_long<T, S, JOIN>), dim3(a.rows < most ? a.rows : most), block, 0, stream, a);
+        if (sums) {
+            hipLaunchKernelGGL((k_norm_bwd_cols_long<T, H>), dim3(ceil_div(units, 256), blocks), dim3(256), 0, stream, a);
+            norm_finish(a, blocks, stream);
+        }
+        return;
+    }
+    if (!s.block && s.nv == 1)
+        hipLaunchKernelGGL((k_norm_bwd<T, S, JOIN, 1, false>), grid, block, 0, stream, a);
+    else if (!s.block)
+        hipLaunchKernelGGL((k_norm_bwd<T, S, JOIN, 2, false>), grid, block, 0, stream, a);
+    else if (s.nv == 1)
+        hipLaunchKernelGGL((k_norm_bwd<T, S, JOIN, 1, true>), grid, block, 0, stream, a);
+    else
+        hipLaunchKernelGGL((k_norm_bwd<T, S, JOIN, 2, true>), grid, block, 0, stream, a);
+    if (sums && blocks > 1) norm_finish(a, blocks, stream);
+}
+
+}  // namespace
+}  // namespace fiery

@@ -13,7 +13,7 @@
  *   - work is enqueued on `stream` (a hipStream_t passed as void*); no call synchronises, allocates
  *     or frees device memory - the caller owns every buffer including workspaces, so calls are
  *     hipGraph-capturable and re-entrant across streams given distinct workspaces;
- *   - fp32 tensors; "NHWC" tensors are addressed as base + image*img_stride + (y*W + x)*ld + channel.
+ *   - fp32 tensors unless the parameter's type is given (FIERY_TYPE_*); "NHWC" tensors are addressed as base + image*img_stride + (y*W + x)*ld + channel.
  */
 #ifndef FIERY_HIP_H
 #define FIERY_HIP_H
@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define FIERY_ABI_VERSION 25      /* 25 (round 6): fiery_conv_desc grew (weights2_split, weights3_split); 24 (round 6): the split Winograd form (fiery_conv_pack_weights_winograd_split, FIERY_CONV_FORM_WINOGRAD_SPLIT); 23 (round 6): fiery_conv_form_used, FIERY_POOL_NO_RANKS, the prepass quantises without divisions where that is exact; 22 (round 5): fiery_conv_desc grew (weights_winograd, winograd, stream_k, sk_*); fiery_conv_pack_weights_winograd, fiery_conv_winograd_packed_floats, fiery_conv_stream_k_plan */
+#define FIERY_ABI_VERSION 26      /* 26: row operators (fiery_layer_norm_*, fiery_dropout, fiery_dropout_add_layer_norm_*); 25 (round 6): fiery_conv_desc grew (weights2_split, weights3_split); 24 (round 6): the split Winograd form (fiery_conv_pack_weights_winograd_split, FIERY_CONV_FORM_WINOGRAD_SPLIT); 23 (round 6): fiery_conv_form_used, FIERY_POOL_NO_RANKS, the prepass quantises without divisions where that is exact; 22 (round 5): fiery_conv_desc grew (weights_winograd, winograd, stream_k, sk_*); fiery_conv_pack_weights_winograd, fiery_conv_winograd_packed_floats, fiery_conv_stream_k_plan */
 
 #define FIERY_OK 0
 #define FIERY_EINVAL (-22)      /* bad argument (shape, alignment, null pointer) */
@@ -543,6 +543,60 @@ int fiery_scale_channels_nhwc(float* x, int ld, int n_img, int HW, int C, const 
 int fiery_upsample2x_add_nhwc(const float* in, int in_ld, int n_img, int H, int W, int C,
                               const float* shift, const float* skip, int skip_ld,
                               float* out, int out_ld, fiery_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Row operators: layer norm, dropout, and residual + dropout + layer norm, forward and backward
+ *
+ * Rows of C elements, `ld` elements between rows (pixel-major activations: one row per pixel).  Element types FIERY_TYPE_*; the
+ * address of an element needs no alignment beyond the type's own.  1 <= rows < 2^31, 1 <= C <= 2^30.  A row stride of an INPUT may
+ * be anything >= 0 (0: every row is the same one); of an output it is at least C, and what lies between its rows stays as it was.
+ * Outputs overlap neither each other nor an input.  Sums and statistics are fp32 or more; a 16-bit result is rounded once.
+ * gamma, beta: C values of fp32 or of the rows' type (param_type), each may be NULL (1 / 0).  Results are deterministic.
+ * ---------------------------------------------------------------------------------------------- */
+#define FIERY_TYPE_F32 0
+#define FIERY_TYPE_BF16 1
+#define FIERY_TYPE_F16 2
+
+/* y = (x - mean) * rstd * gamma + beta with the mean and biased variance of each row, rstd = 1 / sqrt(var + eps).
+ * mean, rstd: [rows] for the backward pass, both or neither NULL. */
+int fiery_layer_norm_fwd(const void* x, int64_t x_ld, int x_type, int64_t rows, int C, const void* gamma, const void* beta, int param_type,
+                         float eps, void* y, int64_t y_ld, float* mean, float* rstd, fiery_stream_t stream);
+/* dx (rows' type), dgamma[C], dbeta[C] (param_type); each may be NULL, not all.  workspace: needed for dgamma / dbeta,
+ * fiery_layer_norm_bwd_workspace_floats(rows, C) floats, contents on entry irrelevant. */
+int64_t fiery_layer_norm_bwd_workspace_floats(int64_t rows, int C);
+int fiery_layer_norm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int x_type, int64_t rows, int C, const void* gamma,
+                         int param_type, const float* mean, const float* rstd, void* dx, int64_t dx_ld, void* dgamma, void* dbeta,
+                         float* workspace, int64_t workspace_floats, fiery_stream_t stream);
+
+/* y = [residual +] (kept ? x * 65536 / (65536 - threshold) : 0).  What is kept is a function of (seed, call, mask row, column):
+ * Philox4x32-10 (Salmon, Moraes, Dror, Shaw 2011) with the counter {column / 8, mask row, call low, call high} and the key
+ * {seed low, seed high} gives four words; column c takes word (c % 8) / 2, its low half where c is even; kept iff that half is at
+ * least `threshold` (0 .. 65536 = round(65536 p); 0: nothing is dropped and rng may be NULL).
+ *   rng: device int64 {seed, call}; `call` below is added to it (one number per dropout of a step).
+ *   rows_per_mask: rows that share one mask row (row / rows_per_mask); one_column: all columns take column 0's number.
+ *     element masks: 1, 0; per channel of images of P pixels (nn.Dropout2d): P, 0; per image (drop-connect): P, 1.
+ *   rng_used: device int64[2] or NULL: receives {seed, call} as used - what the backward pass is given as its rng, with call 0,
+ *     so that a program may advance `rng` in place in between.
+ * residual: y's type or NULL.  x_type and y_type are equal or one of them is fp32.  The gradient of x is this call on the
+ * gradient of y (rng_used, no residual), the gradient of residual is the gradient of y.
+ * rows * ceil(C / 8) < 2^31. */
+int fiery_dropout(const void* x, int64_t x_ld, int x_type, const void* residual, int64_t res_ld, int64_t rows, int C, int threshold,
+                  const int64_t* rng, int64_t call, int64_t rows_per_mask, int one_column, int64_t* rng_used, void* y, int64_t y_ld, int y_type,
+                  fiery_stream_t stream);
+
+/* h = residual + dropout(x), y = layer norm(h): one pass.  residual, h and their gradients are of stream_type (the rows' type or
+ * fp32); y comes from h before it is rounded to that type, mean and rstd are those of the h that is stored, which the backward pass
+ * reads: its gradients are the norm's at that h.  Backward: dh = the gradient of h itself or NULL;
+ * dresidual = dh + d(layer norm), dx = dropout of it; every output may be NULL, not all.  Mask, statistics, workspace: as above. */
+int fiery_dropout_add_layer_norm_fwd(const void* x, int64_t x_ld, int x_type, const void* residual, int64_t res_ld, int stream_type, int64_t rows,
+                                     int C, const void* gamma, const void* beta, int param_type, float eps, int threshold, const int64_t* rng,
+                                     int64_t call, int64_t rows_per_mask, int one_column, int64_t* rng_used, void* y, int64_t y_ld, void* h,
+                                     int64_t h_ld, float* mean, float* rstd, fiery_stream_t stream);
+int fiery_dropout_add_layer_norm_bwd(const void* dy, int64_t dy_ld, const void* dh, int64_t dh_ld, const void* h, int64_t h_ld, int x_type,
+                                     int stream_type, int64_t rows, int C, const void* gamma, int param_type, const float* mean,
+                                     const float* rstd, int threshold, const int64_t* rng_used, int64_t rows_per_mask, int one_column,
+                                     void* dx, int64_t dx_ld, void* dresidual, int64_t dres_ld, void* dgamma, void* dbeta, float* workspace,
+                                     int64_t workspace_floats, fiery_stream_t stream);
 
 /* BatchNorm with batch statistics (+ fused ReLU) on pixel-major rows - what `nn.BatchNorm2d / BatchNorm3d (+ nn.ReLU)` of the
  * BEV stack compute in train() mode (layers/convolutions.py:27-34, 85-105; layers/temporal.py:77-84, 107-117; autograd's

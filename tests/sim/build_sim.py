@@ -16,7 +16,8 @@ def build():
     os.makedirs(OUT_DIR, exist_ok=True)
     deps = [os.path.join(CSRC, n) for n, _ in SOURCES] + [
         os.path.join(CSRC, 'common.h'), os.path.join(CSRC, 'conv_igemm_kernel.h'), os.path.join(ROOT, 'include', 'fiery_hip.h'),
-        os.path.join(HERE, 'include', 'fiery_gfx950.h'),
+        os.path.join(HERE, 'include', 'fiery_gfx950.h'), os.path.join(HERE, 'include', 'fiery_row_types.h'),
+        os.path.join(CSRC, 'row_ops.h'), os.path.join(CSRC, 'layer_norm_kernel.h'),
         os.path.join(HERE, 'include', 'hip', 'hip_runtime.h')]
     if os.path.exists(OUT) and all(os.path.getmtime(d) <= os.path.getmtime(OUT) for d in deps):
         return OUT
