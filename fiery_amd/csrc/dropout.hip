@@ -22,7 +22,7 @@ struct DropoutArgs {
     DropArgs drop;
 };
 
-template <typename I, typename O, bool RES>
+template <typename I, typename O, bool RES, bool RAGGED>
 __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
     DropKey key = {0, 0, 0, 0};
     if (a.drop.threshold) key = drop_key(a.drop);
@@ -30,29 +30,31 @@ __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
     for (unsigned long long q = static_cast<unsigned long long>(blockIdx.x) * 256 + threadIdx.x; q < a.total; q += static_cast<unsigned long long>(gridDim.x) * 256) {
         const unsigned row = div_by(static_cast<unsigned>(q), a.units), unit = static_cast<unsigned>(q) - row * a.units.d;
         const long long c = static_cast<long long>(unit) * kUnit;
-        const int count = static_cast<long long>(a.C) - c >= kUnit ? kUnit : static_cast<int>(a.C - c);
+        const int count = RAGGED ? unit_count<true>(a.C, unit) : kUnit;
         float v[kUnit];
-        load_unit<I>(static_cast<const typename I::store*>(a.x) + row * a.x_ld + c, count, v);
+        load_unit<I, RAGGED>(static_cast<const typename I::store*>(a.x) + row * a.x_ld + c, count, a.C, v);
         if constexpr (RES) {
             float r[kUnit];
-            load_unit<O>(static_cast<const typename O::store*>(a.residual) + row * a.res_ld + c, count, r);
+            load_unit<O, RAGGED>(static_cast<const typename O::store*>(a.residual) + row * a.res_ld + c, count, a.C, r);
             drop_unit(a.drop, key, row, unit, v);
 #pragma unroll
             for (int j = 0; j < kUnit; ++j) v[j] += r[j];
         } else {
             drop_unit(a.drop, key, row, unit, v);
         }
-        store_unit<O>(static_cast<typename O::store*>(a.y) + row * a.y_ld + c, count, v);
+        store_unit<O, RAGGED>(static_cast<typename O::store*>(a.y) + row * a.y_ld + c, count, v);
     }
 }
 
 template <typename I, typename O>
 void dropout_launch(const DropoutArgs& a, hipStream_t stream) {
     const dim3 grid(ceil_div(a.total, 256)), block(256);
+    const bool ragged = a.C % kUnit;
+    const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a); };
     if (a.residual)
-        hipLaunchKernelGGL((k_dropout<I, O, true>), grid, block, 0, stream, a);
+        ragged ? run(k_dropout<I, O, true, true>) : run(k_dropout<I, O, true, false>);
     else
-        hipLaunchKernelGGL((k_dropout<I, O, false>), grid, block, 0, stream, a);
+        ragged ? run(k_dropout<I, O, false, true>) : run(k_dropout<I, O, false, false>);
 }
 
 }  // namespace

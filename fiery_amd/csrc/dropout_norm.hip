@@ -71,7 +71,7 @@ extern "C" int fiery_dropout_add_layer_norm_bwd(const void* dy, int64_t dy_ld, c
     FIERY_REQUIRE(!bad, "dropout_add_layer_norm_bwd: %s", bad);
     FIERY_REQUIRE(dy_ld >= 0 && h_ld >= 0 && (!dh || dh_ld >= 0) && (!dx || dx_ld >= C) && (!dresidual || dres_ld >= C),
                   "dropout_add_layer_norm_bwd: bad row stride");
-    if (dgamma || dbeta) {
+    if ((dgamma || dbeta) && norm_bwd_workspace_floats(rows, C) > 0) {
         FIERY_REQUIRE(workspace, "dropout_add_layer_norm_bwd: null workspace");
         if (workspace_floats < norm_bwd_workspace_floats(rows, C)) return fail(FIERY_ENOMEM, "dropout_add_layer_norm_bwd: workspace too small");
     }

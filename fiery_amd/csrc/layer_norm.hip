@@ -13,6 +13,7 @@ __global__ __launch_bounds__(1024) void k_norm_finish(const float* __restrict__ 
     double s = 0.0;
     if (c < C) {
         const float* p = partial + static_cast<long long>(blockIdx.y) * width + c;
+#pragma unroll 8
         for (int b = r; b < blocks; b += 64) s += p[static_cast<long long>(b) * 2 * width];
     }
     lds[r][col] = s;
@@ -81,7 +82,7 @@ extern "C" int fiery_layer_norm_bwd(const void* dy, int64_t dy_ld, const void* x
     const char* bad = norm_check(rows, C, x_type, param_type, gamma || dgamma || dbeta);
     FIERY_REQUIRE(!bad, "layer_norm_bwd: %s", bad);
     FIERY_REQUIRE(x_ld >= 0 && dy_ld >= 0 && (!dx || dx_ld >= C), "layer_norm_bwd: bad row stride");
-    if (dgamma || dbeta) {
+    if ((dgamma || dbeta) && norm_bwd_workspace_floats(rows, C) > 0) {
         FIERY_REQUIRE(workspace, "layer_norm_bwd: null workspace");
         if (workspace_floats < norm_bwd_workspace_floats(rows, C)) return fail(FIERY_ENOMEM, "layer_norm_bwd: workspace too small");
     }

@@ -8,7 +8,7 @@
 // Memory-bound: every tensor is read once and written once.  A row lives in registers between its load and its store, so the
 // two sums (mean, then squared distances from it: no cancellation) cost no second pass.  A row is dealt to lanes in units of
 // eight columns (row_ops.h): a power-of-two group of up to 64 lanes of one wavefront (C <= 1024, no barrier), a workgroup (up
-// to 32768 forward, 16384 backward), or, past that, a workgroup that walks the row three times.
+// to 8192), or, past that, a workgroup that walks the row three times.
 // The backward pass deals a lane the same columns for all its rows, so dgamma and dbeta grow in registers; every workgroup
 // leaves one partial row and k_norm_finish adds them in a fixed order in double.  Sums and statistics are fp32; what is
 // stored in 16 bits is rounded once, at the store.
@@ -55,26 +55,24 @@ struct NormBwdArgs {
 
 namespace {
 
-__device__ __forceinline__ float lanes_sum(float v, int lanes) {
-    for (int m = 1; m < lanes; m <<= 1) v += __shfl_xor(v, m);
-    return v;
-}
-
-// Sum over the lanes that share a row, the same in all of them.  BLOCK: over the workgroup, through one of two slots used in
+// Sum over the lanes that share a row, the same in all of them.  THREADS > 0: over the workgroup, through one of two slots used in
 // turn (a slot is written again only behind the barrier of the call in between).
-template <bool BLOCK, int N>
-__device__ __forceinline__ void row_sums(float (&v)[N], int lanes, float (*slots)[16][2], int& turn) {
+template <int THREADS, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], int lanes, float (*slots)[2][16], int& turn) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = lanes_sum(v[i], BLOCK ? 64 : lanes);
-    if constexpr (BLOCK) {
-        const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-        if ((threadIdx.x & 63) == 0)
-            for (int i = 0; i < N; ++i) slots[turn][wave][i] = v[i];
+    for (int i = 0; i < N; ++i) v[i] = lanes_sum(v[i], THREADS ? 64 : lanes);
+    if constexpr (THREADS > 0) {
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) slots[turn][i][wave] = v[i];
+        }
         __syncthreads();
+#pragma unroll
         for (int i = 0; i < N; ++i) {
-            float s = 0.f;
-            for (int w = 0; w < waves; ++w) s += slots[turn][w][i];
-            v[i] = s;
+            v[i] = 0.f;
+#pragma unroll
+            for (int w = 0; w < THREADS / 64; ++w) v[i] += slots[turn][i][w];
         }
         turn ^= 1;
     }
@@ -86,26 +84,50 @@ __device__ __forceinline__ float mean_of(float s, int C, float inv_c) {
     return fmaf(fmaf(-m, static_cast<float>(C), s), inv_c, m);
 }
 
-__device__ __forceinline__ int unit_count(int C, int unit) {
-    const int left = C - unit * kUnit;
-    return left >= kUnit ? kUnit : left > 0 ? left : 0;
+// 1 / sqrt(x) of a variance plus eps: the hardware's estimate and one Newton step, or the exact functions at the ends of the range
+__device__ __forceinline__ float rstd_of(float x) {
+    if (!(x > 1e-30f && x < 1e30f)) return 1.f / sqrtf(x);
+    const float r = rsq_estimate(x);
+    return fmaf(r * fmaf(-x * r, r, 1.f), 0.5f, r);
 }
 
 // one unit of h: x alone, or residual + drop(x), written out as it is read
-template <typename T, typename S, bool JOIN>
+template <typename T, typename S, bool JOIN, bool RAGGED>
 __device__ __forceinline__ void load_h(const NormFwdArgs& a, const DropKey& key, long long row, int unit, int count, bool write, float (&v)[kUnit]) {
     const long long c = static_cast<long long>(unit) * kUnit;
-    load_unit<T>(static_cast<const typename T::store*>(a.x) + row * a.x_ld + c, count, v);
-    if constexpr (JOIN) {
+    const Raw<T> x = load_raw<T, RAGGED>(static_cast<const typename T::store*>(a.x) + row * a.x_ld + c, count, a.C);
+    if constexpr (!JOIN) {
+        unpack<T, RAGGED>(x, count, a.C, v);
+    } else {
+        const Raw<S> residual = load_raw<S, RAGGED>(static_cast<const typename S::store*>(a.residual) + row * a.res_ld + c, count, a.C);
         float r[kUnit];
-        load_unit<S>(static_cast<const typename S::store*>(a.residual) + row * a.res_ld + c, count, r);
+        unpack<T, RAGGED>(x, count, a.C, v);
+        unpack<S, RAGGED>(residual, count, a.C, r);
         drop_unit(a.drop, key, static_cast<unsigned>(row), static_cast<unsigned>(unit), v);
 #pragma unroll
         for (int j = 0; j < kUnit; ++j) v[j] += r[j];
-        if (write) store_unit<S>(static_cast<typename S::store*>(a.h) + row * a.h_ld + c, count, v);
+        if (write) store_unit<S, RAGGED>(static_cast<typename S::store*>(a.h) + row * a.h_ld + c, count, v);
     }
 }
 
+template <bool RAGGED>
+__device__ __forceinline__ void distances(const float (&v)[kUnit], int count, float mean, float& q) {
+    if constexpr (RAGGED) {
+#pragma unroll
+        for (int j = 0; j < kUnit; ++j) {
+            const float d = j < count ? v[j] - mean : 0.f;
+            q += d * d;
+        }
+    } else {
+        float p = 0.f;
+#pragma unroll
+        for (int j = 0; j < kUnit; ++j) {
+            const float d = v[j] - mean;
+            p += d * d;
+        }
+        q += count ? p : 0.f;
+    }
+}
 template <typename S>
 __device__ __forceinline__ void sum_stored(const float (&v)[kUnit], float& s) {
     float r[kUnit];
@@ -113,25 +135,14 @@ __device__ __forceinline__ void sum_stored(const float (&v)[kUnit], float& s) {
 #pragma unroll
     for (int j = 0; j < kUnit; ++j) s += r[j];
 }
-template <typename S>
-__device__ __forceinline__ void distances_stored(const float (&v)[kUnit], int count, float mean, float& q) {
-    float r[kUnit];
-    as_stored<S>(v, r);
-#pragma unroll
-    for (int j = 0; j < kUnit; ++j) {
-        const float d = j < count ? r[j] - mean : 0.f;
-        q += d * d;
-    }
-}
-
-template <typename T, typename S, bool JOIN, int NV, bool BLOCK>
-__global__ __launch_bounds__(BLOCK ? 1024 : 256) void k_norm_fwd(NormFwdArgs a) {
-    __shared__ float slots[2][16][2];
+template <typename T, typename S, bool JOIN, int NV, int THREADS, bool RAGGED>
+__global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_fwd(NormFwdArgs a) {
+    __shared__ float slots[2][2][16];
     int turn = 0;
-    const int lanes = BLOCK ? static_cast<int>(blockDim.x) : 1 << a.lane_bits;
+    const int lanes = THREADS ? THREADS : 1 << a.lane_bits;
     const int sub = static_cast<int>(threadIdx.x) & (lanes - 1);
-    const int per_block = BLOCK ? 1 : 256 >> a.lane_bits;
-    const int mine = BLOCK ? 0 : static_cast<int>(threadIdx.x) >> a.lane_bits;
+    const int per_block = THREADS ? 1 : 256 >> a.lane_bits;
+    const int mine = THREADS ? 0 : static_cast<int>(threadIdx.x) >> a.lane_bits;
     DropKey key = {0, 0, 0, 0};
     if constexpr (JOIN) {
         if (a.drop.threshold) key = drop_key(a.drop);
@@ -139,13 +150,11 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void k_norm_fwd(NormFwdArgs a) 
     }
     float ga[NV][kUnit], be[NV][kUnit];
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < kUnit; ++j) {
-            const int c = (i * lanes + sub) * kUnit + j;
-            ga[i][j] = a.gamma && c < a.C ? load_typed(a.gamma, a.param_type, c) : 1.f;
-            be[i][j] = a.beta && c < a.C ? load_typed(a.beta, a.param_type, c) : 0.f;
-        }
+    for (int i = 0; i < NV; ++i) {
+        const int unit = i * lanes + sub, count = unit_count<RAGGED>(a.C, unit);
+        load_typed(a.gamma, a.param_type, static_cast<long long>(unit) * kUnit, count, a.C, 1.f, ga[i]);
+        load_typed(a.beta, a.param_type, static_cast<long long>(unit) * kUnit, count, a.C, 0.f, be[i]);
+    }
     // (every lane of a wavefront walks the loop as often as its neighbours: the exchanges need all of them)
     for (long long first = static_cast<long long>(blockIdx.x) * per_block; first < a.rows; first += static_cast<long long>(gridDim.x) * per_block) {
         const long long row = first + mine;
@@ -157,40 +166,35 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void k_norm_fwd(NormFwdArgs a) 
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int unit = i * lanes + sub;
-            count[i] = live ? unit_count(a.C, unit) : 0;
-            if constexpr (JOIN) {
-                for (int j = 0; j < kUnit; ++j) v[i][j] = 0.f;
-                if (count[i]) load_h<T, S, true>(a, key, row, unit, count[i], true, v[i]);
-            } else {
-                load_h<T, S, false>(a, key, live ? row : 0, unit, count[i], false, v[i]);
-            }
+            count[i] = live ? unit_count<RAGGED>(a.C, unit) : 0;
+            load_h<T, S, JOIN, RAGGED>(a, key, row, unit, count[i], true, v[i]);
 #pragma unroll
             for (int j = 0; j < kUnit; ++j) s[0] += v[i][j];
             if constexpr (two) sum_stored<S>(v[i], s[1]);
         }
-        row_sums<BLOCK>(s, lanes, slots, turn);
+        row_sums<THREADS>(s, lanes, slots, turn);
         const float mean = mean_of(s[0], a.C, a.inv_c);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-#pragma unroll
-            for (int j = 0; j < kUnit; ++j) {
-                const float d = j < count[i] ? v[i][j] - mean : 0.f;
-                q[0] += d * d;
+            distances<RAGGED>(v[i], count[i], mean, q[0]);
+            if constexpr (two) {
+                float r[kUnit];
+                as_stored<S>(v[i], r);
+                distances<RAGGED>(r, count[i], mean_of(s[1], a.C, a.inv_c), q[1]);
             }
-            if constexpr (two) distances_stored<S>(v[i], count[i], mean_of(s[1], a.C, a.inv_c), q[1]);
         }
-        row_sums<BLOCK>(q, lanes, slots, turn);
-        const float rstd = 1.f / sqrtf(q[0] * a.inv_c + a.eps);
+        row_sums<THREADS>(q, lanes, slots, turn);
+        const float rstd = rstd_of(q[0] * a.inv_c + a.eps);
         if (a.mean && live && sub == 0) {
             a.mean[row] = two ? mean_of(s[two ? 1 : 0], a.C, a.inv_c) : mean;
-            a.rstd[row] = two ? 1.f / sqrtf(q[two ? 1 : 0] * a.inv_c + a.eps) : rstd;
+            a.rstd[row] = two ? rstd_of(q[two ? 1 : 0] * a.inv_c + a.eps) : rstd;
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             float out[kUnit];
 #pragma unroll
             for (int j = 0; j < kUnit; ++j) out[j] = (v[i][j] - mean) * rstd * ga[i][j] + be[i][j];
-            store_unit<T>(static_cast<typename T::store*>(a.y) + (live ? row : 0) * a.y_ld + static_cast<long long>(i * lanes + sub) * kUnit, count[i], out);
+            store_unit<T, RAGGED>(static_cast<typename T::store*>(a.y) + row * a.y_ld + static_cast<long long>(i * lanes + sub) * kUnit, count[i], out);
         }
     }
 }
@@ -199,7 +203,7 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void k_norm_fwd(NormFwdArgs a) 
 // third come out of the caches.
 template <typename T, typename S, bool JOIN>
 __global__ __launch_bounds__(1024) void k_norm_fwd_long(NormFwdArgs a) {
-    __shared__ float slots[2][16][2];
+    __shared__ float slots[2][2][16];
     int turn = 0;
     const int units = (a.C + kUnit - 1) / kUnit;
     DropKey key = {0, 0, 0, 0};
@@ -211,47 +215,46 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_long(NormFwdArgs a) {
         constexpr bool two = JOIN && sizeof(typename S::store) == 2;
         float v[kUnit], s[two ? 2 : 1] = {}, q[two ? 2 : 1] = {};
         for (int u = threadIdx.x; u < units; u += blockDim.x) {
-            load_h<T, S, JOIN>(a, key, row, u, unit_count(a.C, u), true, v);
+            load_h<T, S, JOIN, true>(a, key, row, u, unit_count<true>(a.C, u), true, v);
 #pragma unroll
             for (int j = 0; j < kUnit; ++j) s[0] += v[j];
             if constexpr (two) sum_stored<S>(v, s[1]);
         }
-        row_sums<true>(s, 64, slots, turn);
+        row_sums<1024>(s, 64, slots, turn);
         const float mean = mean_of(s[0], a.C, a.inv_c);
         for (int u = threadIdx.x; u < units; u += blockDim.x) {
-            const int count = unit_count(a.C, u);
-            load_h<T, S, JOIN>(a, key, row, u, count, false, v);
-#pragma unroll
-            for (int j = 0; j < kUnit; ++j) {
-                const float d = j < count ? v[j] - mean : 0.f;
-                q[0] += d * d;
+            const int count = unit_count<true>(a.C, u);
+            load_h<T, S, JOIN, true>(a, key, row, u, count, false, v);
+            distances<true>(v, count, mean, q[0]);
+            if constexpr (two) {
+                float r[kUnit];
+                as_stored<S>(v, r);
+                distances<true>(r, count, mean_of(s[1], a.C, a.inv_c), q[1]);
             }
-            if constexpr (two) distances_stored<S>(v, count, mean_of(s[1], a.C, a.inv_c), q[1]);
         }
-        row_sums<true>(q, 64, slots, turn);
-        const float rstd = 1.f / sqrtf(q[0] * a.inv_c + a.eps);
+        row_sums<1024>(q, 64, slots, turn);
+        const float rstd = rstd_of(q[0] * a.inv_c + a.eps);
         if (a.mean && threadIdx.x == 0) {
             a.mean[row] = two ? mean_of(s[two ? 1 : 0], a.C, a.inv_c) : mean;
-            a.rstd[row] = two ? 1.f / sqrtf(q[two ? 1 : 0] * a.inv_c + a.eps) : rstd;
+            a.rstd[row] = two ? rstd_of(q[two ? 1 : 0] * a.inv_c + a.eps) : rstd;
         }
         for (int u = threadIdx.x; u < units; u += blockDim.x) {
-            const int count = unit_count(a.C, u);
-            load_h<T, S, JOIN>(a, key, row, u, count, false, v);
+            const int count = unit_count<true>(a.C, u);
+            load_h<T, S, JOIN, true>(a, key, row, u, count, false, v);
+            float ga[kUnit], be[kUnit];
+            load_typed(a.gamma, a.param_type, static_cast<long long>(u) * kUnit, count, a.C, 1.f, ga);
+            load_typed(a.beta, a.param_type, static_cast<long long>(u) * kUnit, count, a.C, 0.f, be);
 #pragma unroll
-            for (int j = 0; j < kUnit; ++j)
-                if (j < count) {
-                    const long long c = static_cast<long long>(u) * kUnit + j;
-                    v[j] = (v[j] - mean) * rstd * (a.gamma ? load_typed(a.gamma, a.param_type, c) : 1.f) + (a.beta ? load_typed(a.beta, a.param_type, c) : 0.f);
-                }
-            store_unit<T>(static_cast<typename T::store*>(a.y) + row * a.y_ld + static_cast<long long>(u) * kUnit, count, v);
+            for (int j = 0; j < kUnit; ++j) v[j] = (v[j] - mean) * rstd * ga[j] + be[j];
+            store_unit<T, true>(static_cast<typename T::store*>(a.y) + row * a.y_ld + static_cast<long long>(u) * kUnit, count, v);
         }
     }
 }
 
 // One unit of the backward pass's results from its dy (gg = dy gamma), xhat and the row's sums.
-template <typename T, typename S, bool JOIN>
+template <typename T, typename S, bool JOIN, bool RAGGED>
 __device__ __forceinline__ void store_grads(const NormBwdArgs& a, const DropKey& key, long long row, int unit, int count, const float (&gg)[kUnit],
-                                            const float (&xhat)[kUnit], float rstd, float m1, float m2) {
+                                            const float (&xhat)[kUnit], const Raw<S>& dh, float rstd, float m1, float m2) {
     const long long c = static_cast<long long>(unit) * kUnit;
     float out[kUnit];
 #pragma unroll
@@ -259,77 +262,97 @@ __device__ __forceinline__ void store_grads(const NormBwdArgs& a, const DropKey&
     if constexpr (JOIN) {
         if (a.dh) {
             float d[kUnit];
-            load_unit<S>(static_cast<const typename S::store*>(a.dh) + row * a.dh_ld + c, count, d);
+            unpack<S, RAGGED>(dh, count, a.C, d);
 #pragma unroll
             for (int j = 0; j < kUnit; ++j) out[j] += d[j];
         }
-        if (a.dres) store_unit<S>(static_cast<typename S::store*>(a.dres) + row * a.dres_ld + c, count, out);
+        if (a.dres) store_unit<S, RAGGED>(static_cast<typename S::store*>(a.dres) + row * a.dres_ld + c, count, out);
         if (!a.dx) return;
         drop_unit(a.drop, key, static_cast<unsigned>(row), static_cast<unsigned>(unit), out);
     } else {
         if (!a.dx) return;
     }
-    store_unit<T>(static_cast<typename T::store*>(a.dx) + row * a.dx_ld + c, count, out);
+    store_unit<T, RAGGED>(static_cast<typename T::store*>(a.dx) + row * a.dx_ld + c, count, out);
 }
 
-template <typename T, typename S, bool JOIN, int NV, bool BLOCK>
-__global__ __launch_bounds__(BLOCK ? 1024 : 256) void k_norm_bwd(NormBwdArgs a) {
+template <typename T, typename S, bool JOIN, int NV, int THREADS, bool RAGGED>
+__global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_bwd(NormBwdArgs a) {
     typedef typename std::conditional<JOIN, S, T>::type H;
-    __shared__ float slots[2][16][2];
+    __shared__ float slots[2][2][16];
     int turn = 0;
-    const int lanes = BLOCK ? static_cast<int>(blockDim.x) : 1 << a.lane_bits;
+    const int lanes = THREADS ? THREADS : 1 << a.lane_bits;
     const int sub = static_cast<int>(threadIdx.x) & (lanes - 1);
-    const int per_block = BLOCK ? 1 : 256 >> a.lane_bits;
-    const int mine = BLOCK ? 0 : static_cast<int>(threadIdx.x) >> a.lane_bits;
+    const int per_block = THREADS ? 1 : 256 >> a.lane_bits;
+    const int mine = THREADS ? 0 : static_cast<int>(threadIdx.x) >> a.lane_bits;
     DropKey key = {0, 0, 0, 0};
     if constexpr (JOIN)
         if (a.drop.threshold) key = drop_key(a.drop);
     float ga[NV][kUnit], dg[NV][kUnit], db[NV][kUnit];
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+        load_typed(a.gamma, a.param_type, static_cast<long long>(i * lanes + sub) * kUnit, unit_count<RAGGED>(a.C, i * lanes + sub), a.C, 1.f, ga[i]);
 #pragma unroll
-        for (int j = 0; j < kUnit; ++j) {
-            const int c = (i * lanes + sub) * kUnit + j;
-            ga[i][j] = a.gamma && c < a.C ? load_typed(a.gamma, a.param_type, c) : 1.f;
-            dg[i][j] = 0.f;
-            db[i][j] = 0.f;
-        }
-    for (long long first = static_cast<long long>(blockIdx.x) * per_block; first < a.rows; first += static_cast<long long>(gridDim.x) * per_block) {
+        for (int j = 0; j < kUnit; ++j) dg[i][j] = db[i][j] = 0.f;
+    }
+    // the next row's values are on their way while this row's sums go round the lanes
+    const long long step = static_cast<long long>(gridDim.x) * per_block;
+    Raw<H> h_next[NV];
+    Raw<T> g_next[NV];
+    Raw<S> d_next[NV] = {};
+    float mean_next = 0.f, rstd_next = 0.f;
+    const auto fetch = [&](long long first) {
         const long long row = first + mine;
         const bool live = row < a.rows;
         const long long at = live ? row : 0;
-        const float mean = a.mean[at], rstd = a.rstd[at];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int unit = i * lanes + sub, count = live ? unit_count<RAGGED>(a.C, unit) : 0;
+            h_next[i] = load_raw<H, RAGGED>(static_cast<const typename H::store*>(a.h) + at * a.h_ld + static_cast<long long>(unit) * kUnit, count, a.C);
+            g_next[i] = load_raw<T, RAGGED>(static_cast<const typename T::store*>(a.dy) + at * a.dy_ld + static_cast<long long>(unit) * kUnit, count, a.C);
+            if (JOIN && a.dh) d_next[i] = load_raw<S, RAGGED>(static_cast<const typename S::store*>(a.dh) + at * a.dh_ld + static_cast<long long>(unit) * kUnit, count, a.C);
+        }
+        mean_next = live ? a.mean[row] : 0.f;                                      // (a row that is none has xhat 0, whatever row 0 holds)
+        rstd_next = live ? a.rstd[row] : 0.f;
+    };
+    const long long begin = static_cast<long long>(blockIdx.x) * per_block;
+    if (begin < a.rows) fetch(begin);
+    for (long long first = begin; first < a.rows; first += step) {
+        const long long row = first + mine;
+        const bool live = row < a.rows;
+        const long long at = live ? row : 0;
+        const float mean = mean_next, rstd = rstd_next;
         float gg[NV][kUnit], xhat[NV][kUnit], s[2] = {0.f, 0.f};
+        Raw<S> dh[NV];
         int count[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int unit = i * lanes + sub;
-            const long long c = static_cast<long long>(unit) * kUnit;
-            count[i] = live ? unit_count(a.C, unit) : 0;
-            load_unit<H>(static_cast<const typename H::store*>(a.h) + at * a.h_ld + c, count[i], xhat[i]);
-            load_unit<T>(static_cast<const typename T::store*>(a.dy) + at * a.dy_ld + c, count[i], gg[i]);
+            count[i] = live ? unit_count<RAGGED>(a.C, i * lanes + sub) : 0;
+            dh[i] = d_next[i];
+            unpack<H, RAGGED>(h_next[i], count[i], a.C, xhat[i]);
+            unpack<T, RAGGED>(g_next[i], count[i], a.C, gg[i]);
         }
+        if (first + step < a.rows) fetch(first + step);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < kUnit; ++j) {
-                xhat[i][j] = j < count[i] ? (xhat[i][j] - mean) * rstd : 0.f;
+                xhat[i][j] = (xhat[i][j] - mean) * rstd;                           // (past the row gg is 0)
                 dg[i][j] += gg[i][j] * xhat[i][j];
                 db[i][j] += gg[i][j];
                 gg[i][j] *= ga[i][j];
                 s[0] += gg[i][j];
                 s[1] += gg[i][j] * xhat[i][j];
             }
-        row_sums<BLOCK>(s, lanes, slots, turn);
+        row_sums<THREADS>(s, lanes, slots, turn);
         const float m1 = s[0] * a.inv_c, m2 = s[1] * a.inv_c;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (count[i]) store_grads<T, S, JOIN>(a, key, at, i * lanes + sub, count[i], gg[i], xhat[i], rstd, m1, m2);
+            if (count[i]) store_grads<T, S, JOIN, RAGGED>(a, key, at, i * lanes + sub, count[i], gg[i], xhat[i], dh[i], rstd, m1, m2);
     }
     if (!a.partial && !a.dgamma && !a.dbeta) return;
     const int width = (a.C + kUnit - 1) / kUnit * kUnit;
     bool writes = true;
-    if constexpr (!BLOCK) {
+    if constexpr (THREADS == 0) {
         // the lanes that hold the same columns: those of this wavefront, then the other three wavefronts', in order
         __shared__ float others[3][NV * 64 * kUnit][2];
         const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63;
@@ -383,7 +406,7 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void k_norm_bwd(NormBwdArgs a) 
 template <typename T, typename S, bool JOIN>
 __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormBwdArgs a) {
     typedef typename std::conditional<JOIN, S, T>::type H;
-    __shared__ float slots[2][16][2];
+    __shared__ float slots[2][2][16];
     int turn = 0;
     const int units = (a.C + kUnit - 1) / kUnit;
     DropKey key = {0, 0, 0, 0};
@@ -395,14 +418,16 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormBwdArgs a) {
         for (int walk = 0; walk < 2; ++walk) {
             const float m1 = s[0] * a.inv_c, m2 = s[1] * a.inv_c;
             for (int u = threadIdx.x; u < units; u += blockDim.x) {
-                const int count = unit_count(a.C, u);
+                const int count = unit_count<true>(a.C, u);
                 const long long c = static_cast<long long>(u) * kUnit;
-                load_unit<H>(static_cast<const typename H::store*>(a.h) + row * a.h_ld + c, count, xhat);
-                load_unit<T>(static_cast<const typename T::store*>(a.dy) + row * a.dy_ld + c, count, gg);
+                load_unit<H, true>(static_cast<const typename H::store*>(a.h) + row * a.h_ld + c, count, a.C, xhat);
+                load_unit<T, true>(static_cast<const typename T::store*>(a.dy) + row * a.dy_ld + c, count, a.C, gg);
+                float ga[kUnit];
+                load_typed(a.gamma, a.param_type, c, count, a.C, 1.f, ga);
 #pragma unroll
                 for (int j = 0; j < kUnit; ++j) {
-                    xhat[j] = j < count ? (xhat[j] - mean) * rstd : 0.f;
-                    if (a.gamma && j < count) gg[j] *= load_typed(a.gamma, a.param_type, c + j);
+                    xhat[j] = (xhat[j] - mean) * rstd;
+                    gg[j] *= ga[j];
                 }
                 if (walk == 0) {
 #pragma unroll
@@ -411,10 +436,12 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormBwdArgs a) {
                         s[1] += gg[j] * xhat[j];
                     }
                 } else {
-                    store_grads<T, S, JOIN>(a, key, row, u, count, gg, xhat, rstd, m1, m2);
+                    Raw<S> dh = {};
+                    if (JOIN && a.dh) dh = load_raw<S, true>(static_cast<const typename S::store*>(a.dh) + row * a.dh_ld + c, count, a.C);
+                    store_grads<T, S, JOIN, true>(a, key, row, u, count, gg, xhat, dh, rstd, m1, m2);
                 }
             }
-            if (walk == 0) row_sums<true>(s, 64, slots, turn);
+            if (walk == 0) row_sums<1024>(s, 64, slots, turn);
         }
     }
 }
@@ -422,18 +449,18 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormBwdArgs a) {
 // dgamma, dbeta of one unit of columns over the strip blockIdx.y of the rows, one partial row per strip
 template <typename T, typename H>
 __global__ __launch_bounds__(256) void k_norm_bwd_cols_long(NormBwdArgs a) {
-    const int unit = blockIdx.x * 256 + threadIdx.x, count = unit_count(a.C, unit);
+    const int unit = blockIdx.x * 256 + threadIdx.x, count = unit_count<true>(a.C, unit);
     if (count == 0) return;
     const int width = (a.C + kUnit - 1) / kUnit * kUnit;
     const long long c = static_cast<long long>(unit) * kUnit;
     float dg[kUnit] = {}, db[kUnit] = {}, h[kUnit], g[kUnit];
     for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
-        load_unit<H>(static_cast<const typename H::store*>(a.h) + row * a.h_ld + c, count, h);
-        load_unit<T>(static_cast<const typename T::store*>(a.dy) + row * a.dy_ld + c, count, g);
+        load_unit<H, true>(static_cast<const typename H::store*>(a.h) + row * a.h_ld + c, count, a.C, h);
+        load_unit<T, true>(static_cast<const typename T::store*>(a.dy) + row * a.dy_ld + c, count, a.C, g);
         const float mean = a.mean[row], rstd = a.rstd[row];
 #pragma unroll
         for (int j = 0; j < kUnit; ++j) {
-            dg[j] += j < count ? g[j] * ((h[j] - mean) * rstd) : 0.f;
+            dg[j] += g[j] * ((h[j] - mean) * rstd);
             db[j] += g[j];
         }
     }
@@ -454,90 +481,99 @@ inline int row_ops_cus() {
     return n_cu;
 }
 
-// How a row's units are dealt: NV units per lane, `threads` per workgroup, block = the workgroup shares the row; NV 0: long rows.
+// How a row's units are dealt: NV units per lane; threads > 0: a workgroup of that many shares the row; 0: 1 << lane_bits lanes of a
+// wavefront do, in workgroups of 256; nv 0: long rows (1024 threads).
 struct NormShape {
     int nv, threads, lane_bits;
-    bool block;
-    int per_block;                       // rows of one pass of a workgroup
+    int per_block() const { return threads || !nv ? 1 : 256 >> lane_bits; }          // rows of one pass of a workgroup
+    int block() const { return threads ? threads : nv ? 256 : 1024; }
 };
-inline NormShape norm_shape(int C, bool backward) {
+inline NormShape norm_shape(int C) {
     const int units = (C + kUnit - 1) / kUnit;
     if (units <= 128) {
         int bits = 0;
         while (bits < 6 && (1 << bits) < units) ++bits;
-        return {units <= 64 ? 1 : 2, 256, bits, false, 256 >> bits};
+        return {units <= 64 ? 1 : 2, 0, bits};
     }
-    // 128 registers per lane at 1024 threads: forward holds 3 x 8 values a unit at most, backward 5 x 8
-    const int most = backward ? 2 : 4;
-    for (int nv = 1; nv <= most; nv *= 2)
-        for (int threads = 256; threads <= 1024; threads *= 2)
-            if (units <= nv * threads && (nv == most || threads <= 256 * nv)) return {nv, threads, 0, true, 1};
-    return {0, 1024, 0, true, 1};
+    if (units <= 256) return {1, 256, 0};
+    if (units <= 512) return {2, 256, 0};
+    if (units <= 1024) return {2, 512, 0};
+    return {0, 0, 0};
+}
+// at most `most` workgroups, each with as many passes as the others or one less
+inline int even_blocks(int64_t passes, int64_t most) {
+    const int64_t rounds = (passes + most - 1) / most;
+    return static_cast<int>((passes + rounds - 1) / rounds);
 }
 // workgroups of the backward pass = partial rows of dgamma / dbeta
 inline int norm_bwd_blocks(int64_t rows, int C) {
-    const NormShape s = norm_shape(C, true);
+    const NormShape s = norm_shape(C);
     if (s.nv == 0) return static_cast<int>(rows < 16 ? rows : 16);
-    const int64_t passes = (rows + s.per_block - 1) / s.per_block;
-    if (passes <= 2) return 1;
-    const int64_t most = static_cast<int64_t>(row_ops_cus()) * (s.block ? 1024 / s.threads : 4);
-    return static_cast<int>(passes < most ? passes : most);
+    const int64_t passes = (rows + s.per_block() - 1) / s.per_block();
+    if (passes <= 4) return 1;                                               // one workgroup writes the results itself
+    return even_blocks(passes, static_cast<int64_t>(row_ops_cus()) * (s.threads ? (s.threads < 512 ? 512 / s.threads : 1) : 4));
 }
 inline int64_t norm_bwd_workspace_floats(int64_t rows, int C) {
-    return static_cast<int64_t>(norm_bwd_blocks(rows, C)) * 2 * ((C + kUnit - 1) / kUnit * kUnit);
+    const int blocks = norm_bwd_blocks(rows, C);
+    if (blocks == 1 && norm_shape(C).nv) return 0;
+    return static_cast<int64_t>(blocks) * 2 * ((C + kUnit - 1) / kUnit * kUnit);
 }
 
 void norm_finish(const NormBwdArgs& a, int blocks, hipStream_t stream);          // layer_norm.hip
 
 namespace {
 
+template <typename T, typename S, bool JOIN, bool RAGGED, typename Run>
+void norm_fwd_pick(const NormShape& s, Run run) {
+    if (s.threads == 0)
+        s.nv == 1 ? run(k_norm_fwd<T, S, JOIN, 1, 0, RAGGED>) : run(k_norm_fwd<T, S, JOIN, 2, 0, RAGGED>);
+    else if (s.threads == 256)
+        s.nv == 1 ? run(k_norm_fwd<T, S, JOIN, 1, 256, RAGGED>) : run(k_norm_fwd<T, S, JOIN, 2, 256, RAGGED>);
+    else
+        run(k_norm_fwd<T, S, JOIN, 2, 512, RAGGED>);
+}
 template <typename T, typename S, bool JOIN>
 void norm_fwd_launch(NormFwdArgs a, hipStream_t stream) {
-    const NormShape s = norm_shape(a.C, false);
+    const NormShape s = norm_shape(a.C);
     a.lane_bits = s.lane_bits;
-    const long long passes = (static_cast<long long>(a.rows) + s.per_block - 1) / s.per_block;
-    const long long most = static_cast<long long>(row_ops_cus()) * (s.block ? 16384 / s.threads : 64);
-    const dim3 grid(static_cast<unsigned>(passes < most ? passes : most)), block(s.threads);
+    const int64_t passes = (static_cast<int64_t>(a.rows) + s.per_block() - 1) / s.per_block();
+    // as many workgroups as are resident at once: the parameters are read once per workgroup
+    const dim3 grid(even_blocks(passes, static_cast<int64_t>(row_ops_cus()) * (2048 / s.block()))), block(s.block());
+    const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a); };
     if (s.nv == 0)
-        hipLaunchKernelGGL((k_norm_fwd_long<T, S, JOIN>), grid, block, 0, stream, a);
-    else if (!s.block && s.nv == 1)
-        hipLaunchKernelGGL((k_norm_fwd<T, S, JOIN, 1, false>), grid, block, 0, stream, a);
-    else if (!s.block)
-        hipLaunchKernelGGL((k_norm_fwd<T, S, JOIN, 2, false>), grid, block, 0, stream, a);
-    else if (s.nv == 1)
-        hipLaunchKernelGGL((k_norm_fwd<T, S, JOIN, 1, true>), grid, block, 0, stream, a);
-    else if (s.nv == 2)
-        hipLaunchKernelGGL((k_norm_fwd<T, S, JOIN, 2, true>), grid, block, 0, stream, a);
+        run(k_norm_fwd_long<T, S, JOIN>);
     else
-        hipLaunchKernelGGL((k_norm_fwd<T, S, JOIN, 4, true>), grid, block, 0, stream, a);
+        a.C % kUnit ? norm_fwd_pick<T, S, JOIN, true>(s, run) : norm_fwd_pick<T, S, JOIN, false>(s, run);
 }
 
+template <typename T, typename S, bool JOIN, bool RAGGED, typename Run>
+void norm_bwd_pick(const NormShape& s, Run run) {
+    if (s.threads == 0)
+        s.nv == 1 ? run(k_norm_bwd<T, S, JOIN, 1, 0, RAGGED>) : run(k_norm_bwd<T, S, JOIN, 2, 0, RAGGED>);
+    else if (s.threads == 256)
+        s.nv == 1 ? run(k_norm_bwd<T, S, JOIN, 1, 256, RAGGED>) : run(k_norm_bwd<T, S, JOIN, 2, 256, RAGGED>);
+    else
+        run(k_norm_bwd<T, S, JOIN, 2, 512, RAGGED>);
+}
 template <typename T, typename S, bool JOIN>
 void norm_bwd_launch(NormBwdArgs a, hipStream_t stream) {
     typedef typename std::conditional<JOIN, S, T>::type H;
-    const NormShape s = norm_shape(a.C, true);
+    const NormShape s = norm_shape(a.C);
     a.lane_bits = s.lane_bits;
     const bool sums = a.dgamma || a.dbeta;
     const int blocks = norm_bwd_blocks(a.rows, a.C);
     if (!sums) a.partial = nullptr;
-    const dim3 grid(blocks), block(s.threads);
     if (s.nv == 0) {
         const int units = (a.C + kUnit - 1) / kUnit, most = 2 * row_ops_cus();
-        hipLaunchKernelGGL((k_norm_bwd_long<T, S, JOIN>), dim3(a.rows < most ? a.rows : most), block, 0, stream, a);
-        if (sums) {
-            hipLaunchKernelGGL((k_norm_bwd_cols_long<T, H>), dim3(ceil_div(units, 256), blocks), dim3(256), 0, stream, a);
-            norm_finish(a, blocks, stream);
-        }
+        hipLaunchKernelGGL((k_norm_bwd_long<T, S, JOIN>), dim3(a.rows < most ? a.rows : most), dim3(1024), 0, stream, a);
+        if (!sums) return;
+        hipLaunchKernelGGL((k_norm_bwd_cols_long<T, H>), dim3(ceil_div(units, 256), blocks), dim3(256), 0, stream, a);
+        norm_finish(a, blocks, stream);
         return;
     }
-    if (!s.block && s.nv == 1)
-        hipLaunchKernelGGL((k_norm_bwd<T, S, JOIN, 1, false>), grid, block, 0, stream, a);
-    else if (!s.block)
-        hipLaunchKernelGGL((k_norm_bwd<T, S, JOIN, 2, false>), grid, block, 0, stream, a);
-    else if (s.nv == 1)
-        hipLaunchKernelGGL((k_norm_bwd<T, S, JOIN, 1, true>), grid, block, 0, stream, a);
-    else
-        hipLaunchKernelGGL((k_norm_bwd<T, S, JOIN, 2, true>), grid, block, 0, stream, a);
+    const dim3 grid(blocks), block(s.block());
+    const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a); };
+    a.C % kUnit ? norm_bwd_pick<T, S, JOIN, true>(s, run) : norm_bwd_pick<T, S, JOIN, false>(s, run);
     if (sums && blocks > 1) norm_finish(a, blocks, stream);
 }
 

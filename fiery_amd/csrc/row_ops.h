@@ -3,8 +3,7 @@
 //
 // A row's columns are dealt to lanes in UNITS of eight: 16 bytes of a 16-bit type, 32 of fp32, and exactly the columns that one
 // call of the generator serves.  Addresses need no alignment beyond the element's (gfx950's global accesses take any), so odd
-// widths and row strides use the same wide accesses; only the last unit of a row whose width is not a multiple of eight goes
-// in pieces of four, two and one.
+// widths and row strides use the same wide accesses.
 #pragma once
 #include <fiery_row_types.h>
 
@@ -51,28 +50,6 @@ __device__ __forceinline__ void as_stored(const float (&v)[kUnit], float (&out)[
     }
 }
 
-// N consecutive elements (8, 4, 2 or 1), any alignment of the element's own
-template <typename T, int N>
-__device__ __forceinline__ void load_n(const typename T::store* p, float* v) {
-    if constexpr (sizeof(typename T::store) == 4) {
-        if constexpr (N == 8) {
-            __builtin_memcpy(v, p, 16);
-            __builtin_memcpy(v + 4, p + 4, 16);
-        } else {
-            __builtin_memcpy(v, p, 4 * N);
-        }
-    } else if constexpr (N == 1) {
-        v[0] = T::value(p[0]);
-    } else {
-        unsigned w[N / 2];
-        __builtin_memcpy(w, p, 2 * N);
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i) {
-            v[2 * i] = T::value(w[i] & 0xffffu);
-            v[2 * i + 1] = T::value(w[i] >> 16);
-        }
-    }
-}
 template <typename T, int N>
 __device__ __forceinline__ void store_n(typename T::store* p, const float* v) {
     if constexpr (sizeof(typename T::store) == 4) {
@@ -92,53 +69,127 @@ __device__ __forceinline__ void store_n(typename T::store* p, const float* v) {
     }
 }
 
-// The first `count` (0 .. 8) of a unit's elements; the others come out as zeros.  Nothing past them is touched.
-template <typename T>
-__device__ __forceinline__ void load_unit(const typename T::store* p, int count, float (&v)[kUnit]) {
-    if (count == kUnit) {
-        load_n<T, 8>(p, v);
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < kUnit; ++j) v[j] = 0.f;
-    if (count <= 0) return;
-    float four[4] = {0.f, 0.f, 0.f, 0.f}, two[2] = {0.f, 0.f}, one[1] = {0.f};
-    if (count & 4) load_n<T, 4>(p, four);
-    if (count & 2) load_n<T, 2>(p + (count & 4), two);
-    if (count & 1) load_n<T, 1>(p + (count & 6), one);
-    const bool h4 = count & 4, h2 = count & 2;
-    v[0] = h4 ? four[0] : h2 ? two[0] : one[0];
-    v[1] = h4 ? four[1] : h2 ? two[1] : 0.f;
-    v[2] = h4 ? four[2] : h2 ? one[0] : 0.f;
-    v[3] = four[3];
-    v[4] = h4 ? (h2 ? two[0] : one[0]) : 0.f;
-    v[5] = h4 && h2 ? two[1] : 0.f;
-    v[6] = h4 && h2 ? one[0] : 0.f;
+// (values, not references: a conditional of two array elements is a conditional address, which keeps the array out of registers)
+template <typename V>
+__device__ __forceinline__ V pick(bool first, V a, V b) {
+    return first ? a : b;
+}
+
+// A unit as it lies in memory: loads are issued well before unpack() makes their values.  `count` (0 .. 8) of its columns belong
+// to the row, the others come out as zeros and nothing past them is touched.  A last unit with fewer than eight is read as the
+// row's last eight columns, so every lane makes the same access, and shifted into place by unpack(); rows narrower than a unit
+// go in pieces.  RAGGED: the width is no multiple of eight; otherwise none of this is compiled in.
+template <bool RAGGED>
+__device__ __forceinline__ int unit_count(int C, long long unit) {
+    const long long left = C - unit * kUnit;
+    return left >= kUnit ? kUnit : RAGGED && left > 0 ? static_cast<int>(left) : 0;
 }
 template <typename T>
+struct Raw {
+    unsigned w[sizeof(typename T::store) * kUnit / 4];
+};
+template <typename T>
+__device__ __forceinline__ Raw<T> load_pieces(const typename T::store* p, int count) {
+    constexpr int kWords = sizeof(typename T::store) * kUnit / 4;
+    Raw<T> r = {};
+    const bool h4 = count & 4, h2 = count & 2;
+    unsigned four[kWords / 2] = {}, two[kWords / 4] = {}, one = 0;
+    if (h4) __builtin_memcpy(four, p, sizeof(four));
+    if (h2) __builtin_memcpy(two, p + (count & 4), sizeof(two));
+    if (count & 1) {
+        typename T::store e = p[count & 6];
+        if constexpr (sizeof(e) == 4)
+            __builtin_memcpy(&one, &e, 4);
+        else
+            one = e;
+    }
+    if constexpr (sizeof(typename T::store) == 4) {
+        r.w[0] = pick(h4, four[0], pick(h2, two[0], one));
+        r.w[1] = pick(h4, four[1], two[1]);
+        r.w[2] = pick(h4, four[2], pick(h2, one, 0u));
+        r.w[3] = four[3];
+        r.w[4] = pick(h4, pick(h2, two[0], one), 0u);
+        r.w[5] = pick(h4, two[1], 0u);
+        r.w[6] = pick(h4 && h2, one, 0u);
+    } else {
+        r.w[0] = pick(h4, four[0], pick(h2, two[0], one));
+        r.w[1] = pick(h4, four[1], pick(h2, one, 0u));
+        r.w[2] = pick(h4, pick(h2, two[0], one), 0u);
+        r.w[3] = pick(h4 && h2, one, 0u);
+    }
+    return r;
+}
+template <typename T, bool RAGGED>
+__device__ __forceinline__ Raw<T> load_raw(const typename T::store* p, int count, int C) {
+    if (RAGGED && C < kUnit) return load_pieces<T>(p, count);
+    Raw<T> r = {};
+    if (count > 0) {
+        if (RAGGED) p -= kUnit - count;
+        __builtin_memcpy(&r.w[0], p, 16);
+        if constexpr (sizeof(typename T::store) == 4) __builtin_memcpy(&r.w[4], p + 4, 16);
+    }
+    return r;
+}
+template <typename T, bool RAGGED>
+__device__ __forceinline__ void unpack(Raw<T> r, int count, int C, float (&v)[kUnit]) {
+    constexpr int kWords = sizeof(typename T::store) * kUnit / 4;
+    if (RAGGED && C > kUnit) {
+        const unsigned off = count > 0 ? kUnit - count : 0;
+        unsigned words = off;
+        if constexpr (kWords == 4) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) r.w[i] = funnel_halves(i + 1 < kWords ? r.w[i + 1] : 0u, r.w[i], off & 1u);
+            words >>= 1;
+        }
+#pragma unroll
+        for (int step = kWords / 2; step > 0; step >>= 1)
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) r.w[i] = pick((words & step) != 0, i + step < kWords ? r.w[i + step] : 0u, r.w[i]);
+    }
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j) {
+        if constexpr (kWords == 8)
+            __builtin_memcpy(&v[j], &r.w[j], 4);
+        else
+            v[j] = T::value(j & 1 ? r.w[j / 2] >> 16 : r.w[j / 2] & 0xffffu);
+    }
+}
+template <typename T, bool RAGGED>
+__device__ __forceinline__ void load_unit(const typename T::store* p, int count, int C, float (&v)[kUnit]) {
+    unpack<T, RAGGED>(load_raw<T, RAGGED>(p, count, C), count, C, v);
+}
+// (a store of less than a unit goes in pieces)
+template <typename T, bool RAGGED>
 __device__ __forceinline__ void store_unit(typename T::store* p, int count, const float (&v)[kUnit]) {
-    if (count == kUnit) {
+    if (RAGGED ? count == kUnit : count > 0) {
         store_n<T, 8>(p, v);
         return;
     }
-    if (count <= 0) return;
+    if (!RAGGED || count <= 0) return;
     const bool h4 = count & 4, h2 = count & 2;
     if (h4) store_n<T, 4>(p, v);
     if (h2) {
-        const float two[2] = {h4 ? v[4] : v[0], h4 ? v[5] : v[1]};
+        const float two[2] = {pick(h4, v[4], v[0]), pick(h4, v[5], v[1])};
         store_n<T, 2>(p + (count & 4), two);
     }
     if (count & 1) {
-        const float one[1] = {h4 ? (h2 ? v[6] : v[4]) : (h2 ? v[2] : v[0])};
+        const float one[1] = {pick(h4, pick(h2, v[6], v[4]), pick(h2, v[2], v[0]))};
         store_n<T, 1>(p + (count & 6), one);
     }
 }
 
-// one element of a tensor whose type is known at run time (parameters: read once per lane, outside the loops)
-__device__ __forceinline__ float load_typed(const void* p, int type, long long i) {
-    if (type == FIERY_TYPE_F32) return static_cast<const float*>(p)[i];
-    const unsigned b = static_cast<const unsigned short*>(p)[i];
-    return type == FIERY_TYPE_BF16 ? BF16::value(b) : F16::value(b);
+// parameters, whose type is known at run time only: read once per lane, outside the loops
+__device__ __forceinline__ void load_typed(const void* p, int type, long long c, int count, int C, float otherwise, float (&v)[kUnit]) {
+    if (!p) {
+#pragma unroll
+        for (int j = 0; j < kUnit; ++j) v[j] = otherwise;
+    } else if (type == FIERY_TYPE_F32) {
+        load_unit<F32, true>(static_cast<const float*>(p) + c, count, C, v);
+    } else if (type == FIERY_TYPE_BF16) {
+        load_unit<BF16, true>(static_cast<const unsigned short*>(p) + c, count, C, v);
+    } else {
+        load_unit<F16, true>(static_cast<const unsigned short*>(p) + c, count, C, v);
+    }
 }
 __device__ __forceinline__ void store_typed(void* p, int type, long long i, float v) {
     if (type == FIERY_TYPE_F32)
@@ -214,28 +265,19 @@ __device__ __forceinline__ uint4 philox(unsigned c0, unsigned c1, unsigned c2, u
     r.w = c3;
     return r;
 }
-// bit j of the result: column 8 * unit + j of the row is kept
-__device__ __forceinline__ unsigned drop_bits(const DropArgs& d, const DropKey& k, unsigned row, unsigned unit) {
-    const unsigned mask_row = d.rows_per_mask.d > 1 ? div_by(row, d.rows_per_mask) : row;
-    const uint4 w = philox(d.one_column ? 0u : unit, mask_row, k.call_lo, k.call_hi, k.seed_lo, k.seed_hi);
-    if (d.one_column) return (w.x & 0xffffu) >= d.threshold ? 0xffu : 0u;
-    unsigned bits = 0;
-    bits |= (w.x & 0xffffu) >= d.threshold ? 1u : 0u;
-    bits |= (w.x >> 16) >= d.threshold ? 2u : 0u;
-    bits |= (w.y & 0xffffu) >= d.threshold ? 4u : 0u;
-    bits |= (w.y >> 16) >= d.threshold ? 8u : 0u;
-    bits |= (w.z & 0xffffu) >= d.threshold ? 16u : 0u;
-    bits |= (w.z >> 16) >= d.threshold ? 32u : 0u;
-    bits |= (w.w & 0xffffu) >= d.threshold ? 64u : 0u;
-    bits |= (w.w >> 16) >= d.threshold ? 128u : 0u;
-    return bits;
-}
-// (a select and not a product: a dropped infinity or NaN leaves a zero)
+// One unit of a row.  (A select and not a product: a dropped infinity or NaN leaves a zero.  Each half is compared in the upper
+// half of a word, with 65536 threshold - 1: 2^32 - 1 where everything is dropped.)
 __device__ __forceinline__ void drop_unit(const DropArgs& d, const DropKey& k, unsigned row, unsigned unit, float (&v)[kUnit]) {
     if (d.threshold == 0) return;
-    const unsigned bits = drop_bits(d, k, row, unit);
+    const unsigned mask_row = d.rows_per_mask.d > 1 ? div_by(row, d.rows_per_mask) : row;
+    uint4 w = philox(d.one_column ? 0u : unit, mask_row, k.call_lo, k.call_hi, k.seed_lo, k.seed_hi);
+    if (d.one_column) {
+        w.x = (w.x << 16) | (w.x & 0xffffu);
+        w.y = w.z = w.w = w.x;
+    }
+    const unsigned word[4] = {w.x, w.y, w.z, w.w}, limit = d.threshold * 65536u - 1u;
 #pragma unroll
-    for (int j = 0; j < kUnit; ++j) v[j] = (bits >> j) & 1u ? v[j] * d.scale : 0.f;
+    for (int j = 0; j < kUnit; ++j) v[j] = (j & 1 ? word[j / 2] : word[j / 2] << 16) > limit ? v[j] * d.scale : 0.f;
 }
 
 // host side: the arguments of one call, or an error text

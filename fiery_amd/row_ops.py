@@ -69,13 +69,21 @@ def _lib_for(lib, x):
 
 def _launch(lib, x, entry, *args):
     """`entry(*args, stream)` on x's device and its current stream."""
-    if not x.is_cuda:
-        return lib.check(entry(*args, None))
-    dev = x.device.index
-    if dev == torch.cuda.current_device():
-        return lib.check(entry(*args, torch._C._cuda_getCurrentRawStream(dev)))
-    with torch.cuda.device(dev):
-        return lib.check(entry(*args, torch._C._cuda_getCurrentRawStream(dev)))
+    dev = x.get_device()
+    if dev < 0:                                                  # the simulator's library, on host tensors
+        rc = entry(*args, None)
+    elif dev == torch._C._cuda_getDevice():
+        rc = entry(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = entry(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        lib.check(rc)
+
+
+def _new(t, dtype=None):
+    """A dense tensor of t's shape, uninitialised."""
+    return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else torch.empty(t.shape, dtype=dtype or t.dtype, device=t.device)
 
 
 def _ptr(t):
@@ -137,18 +145,19 @@ def _mask_args(x, p, rng, call, per, what):
     return threshold, max(1, rows // max(1, x.shape[0])), int(per == 'sample')
 
 
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
+def _once(grads, ctx, *args):
+    """The gradients, refusing gradients of gradients; the check costs nothing where no graph of the backward pass is made."""
+    return once_differentiable(grads)(ctx, *args) if torch.is_grad_enabled() else grads(ctx, *args)
 
 
 # ---- layer norm -----------------------------------------------------------------------------------------------------------
 def _norm_fwd(lib, x, weight, bias, eps, keep):
     rows, c = _sizes(x)
     xr, ld = _rows(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _new(x)
     if keep:
-        stats = torch.empty(2, rows, dtype=torch.float32, device=x.device)
+        stats = torch.empty(2 * rows, dtype=torch.float32, device=x.device)        # mean, then rstd
         mean = stats.data_ptr()
         rstd = mean + 4 * rows
     else:
@@ -162,7 +171,7 @@ def _norm_fwd(lib, x, weight, bias, eps, keep):
 
 def _param_grads(ctx, weight, bias, first, like):
     """Buffers for the parameters' gradients where they are wanted: (dweight, dbias, type)."""
-    dw = torch.empty(weight.shape, dtype=weight.dtype, device=like.device) if ctx.needs_input_grad[first] else None
+    dw = _new(weight) if ctx.needs_input_grad[first] else None
     db = torch.empty(bias[0], dtype=bias[1], device=like.device) if ctx.needs_input_grad[first + 1] else None
     kind = weight.dtype if weight is not None else bias[1] if bias is not None else torch.float32
     return dw, db, _TYPES[kind]
@@ -170,7 +179,7 @@ def _param_grads(ctx, weight, bias, first, like):
 
 def _workspace(lib, rows, c, like):
     n = lib.dll.fiery_layer_norm_bwd_workspace_floats(rows, c)
-    return torch.empty(n, dtype=torch.float32, device=like.device), n
+    return (torch.empty(n, dtype=torch.float32, device=like.device) if n else None), n
 
 
 class HipLayerNorm(torch.autograd.Function):
@@ -184,12 +193,15 @@ class HipLayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        return _once(HipLayerNorm._grads, ctx, dy)
+
+    @staticmethod
+    def _grads(ctx, dy):
         xr, weight, stats = ctx.saved_tensors
         ld, bias, lib = ctx.meta
         rows, c = _sizes(xr)
-        dx = torch.empty(xr.shape, dtype=xr.dtype, device=xr.device) if ctx.needs_input_grad[0] else None
+        dx = _new(xr) if ctx.needs_input_grad[0] else None
         dw, db, kind = _param_grads(ctx, weight, bias, 1, xr)
         if not rows:
             return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None, None
@@ -208,7 +220,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, lib=None):
     _check_params(x, weight, bias, 'layer_norm')
     lib = _lib_for(lib, x)
     weight, bias = _dense(weight), _dense(bias)
-    if _wants_grad(x, weight, bias):
+    if torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad or bias is not None and bias.requires_grad):
         return HipLayerNorm.apply(x, weight, bias, eps, lib)
     return _norm_fwd(lib, x, weight, bias, eps, False)[0]
 
@@ -220,7 +232,7 @@ def _dense(t):
 # ---- dropout --------------------------------------------------------------------------------------------------------------
 def _dropout(lib, x, residual, out_type, mask, rng, call, used):
     rows, c = _sizes(x)
-    y = torch.empty(x.shape, dtype=out_type, device=x.device)
+    y = _new(x, out_type)
     if rows:
         xr, ld = _rows(x)
         rr, r_ld = (None, 0) if residual is None else _rows(residual)
@@ -242,8 +254,11 @@ class HipDropout(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        return _once(HipDropout._grads, ctx, dy)
+
+    @staticmethod
+    def _grads(ctx, dy):
         used, = ctx.saved_tensors
         dtype, mask, lib = ctx.meta
         dx = _dropout(lib, dy, None, dtype, mask, used, 0, None) if ctx.needs_input_grad[0] else None
@@ -261,7 +276,7 @@ def dropout(x, p, rng=None, *, call=0, per='element', residual=None, lib=None):
         _check_residual(x, residual, 'dropout')
     mask = _mask_args(x, p, rng, call, per, 'dropout')
     lib = _lib_for(lib, x)
-    if _wants_grad(x, residual):
+    if torch.is_grad_enabled() and (x.requires_grad or residual is not None and residual.requires_grad):
         return HipDropout.apply(x, residual, mask, rng, call, lib)
     return _dropout(lib, x, residual, x.dtype if residual is None else residual.dtype, mask, rng, call, None)
 
@@ -269,12 +284,11 @@ def dropout(x, p, rng=None, *, call=0, per='element', residual=None, lib=None):
 # ---- residual + dropout + layer norm ----------------------------------------------------------------------------------------
 def _join_fwd(lib, x, residual, weight, bias, mask, rng, call, eps, keep):
     rows, c = _sizes(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    h = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+    y, h = _new(x), _new(x, residual.dtype)
     threshold, share, one = mask
     stats = used = mean = rstd = None
     if keep:
-        stats = torch.empty(2, rows, dtype=torch.float32, device=x.device)
+        stats = torch.empty(2 * rows, dtype=torch.float32, device=x.device)        # mean, then rstd
         mean = stats.data_ptr()
         rstd = mean + 4 * rows
         if threshold:
@@ -301,8 +315,11 @@ class HipDropoutAddLayerNorm(torch.autograd.Function):
         return y, h
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dh):
+        return _once(HipDropoutAddLayerNorm._grads, ctx, dy, dh)
+
+    @staticmethod
+    def _grads(ctx, dy, dh):
         h, weight, stats, used = ctx.saved_tensors
         dtype, bias, mask, lib = ctx.meta
         rows, c = _sizes(h)
@@ -312,8 +329,8 @@ class HipDropoutAddLayerNorm(torch.autograd.Function):
             dx = _dropout(lib, dh, None, dtype, mask, used, 0, None) if ctx.needs_input_grad[0] and dh is not None else None
             return (dx, dh if ctx.needs_input_grad[1] else None, none(2, None if weight is None else (weight.shape, weight.dtype)), none(3, bias),
                     None, None, None, None, None)
-        dx = torch.empty(h.shape, dtype=dtype, device=h.device) if ctx.needs_input_grad[0] else None
-        dr = torch.empty(h.shape, dtype=h.dtype, device=h.device) if ctx.needs_input_grad[1] else None
+        dx = _new(h, dtype) if ctx.needs_input_grad[0] else None
+        dr = _new(h) if ctx.needs_input_grad[1] else None
         dw, db, kind = _param_grads(ctx, weight, bias, 2, h)
         if not rows:
             return dx, dr, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None, None, None, None, None
@@ -336,6 +353,7 @@ def dropout_add_layer_norm(x, residual, weight=None, bias=None, p=0.0, rng=None,
     mask = _mask_args(x, p, rng, call, per, 'dropout_add_layer_norm')
     lib = _lib_for(lib, x)
     weight, bias = _dense(weight), _dense(bias)
-    if _wants_grad(x, residual, weight, bias):
+    if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or weight is not None and weight.requires_grad or
+                                    bias is not None and bias.requires_grad):
         return HipDropoutAddLayerNorm.apply(x, residual, weight, bias, mask, rng, call, eps, lib)
     return _join_fwd(lib, x, residual, weight, bias, mask, rng, call, eps, False)[:2]

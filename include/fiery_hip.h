@@ -562,7 +562,7 @@ int fiery_upsample2x_add_nhwc(const float* in, int in_ld, int n_img, int H, int 
 int fiery_layer_norm_fwd(const void* x, int64_t x_ld, int x_type, int64_t rows, int C, const void* gamma, const void* beta, int param_type,
                          float eps, void* y, int64_t y_ld, float* mean, float* rstd, fiery_stream_t stream);
 /* dx (rows' type), dgamma[C], dbeta[C] (param_type); each may be NULL, not all.  workspace: needed for dgamma / dbeta,
- * fiery_layer_norm_bwd_workspace_floats(rows, C) floats, contents on entry irrelevant. */
+ * fiery_layer_norm_bwd_workspace_floats(rows, C) floats (0: NULL will do), contents on entry irrelevant. */
 int64_t fiery_layer_norm_bwd_workspace_floats(int64_t rows, int C);
 int fiery_layer_norm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int x_type, int64_t rows, int C, const void* gamma,
                          int param_type, const float* mean, const float* rstd, void* dx, int64_t dx_ld, void* dgamma, void* dbeta,

@@ -33,4 +33,13 @@ inline unsigned bf16_one_bits(float f) {
 }
 inline unsigned bf16_pair_bits(float lo, float hi) { return bf16_one_bits(lo) | (bf16_one_bits(hi) << 16); }
 
+inline float lanes_sum(float v, int lanes) {
+    for (int m = 1; m < lanes; m <<= 1) v += __shfl_xor(v, m);
+    return v;
+}
+inline float rsq_estimate(float x) { return 1.0f / std::sqrt(x); }
+inline unsigned funnel_halves(unsigned hi, unsigned lo, unsigned halves) {
+    return static_cast<unsigned>(((static_cast<unsigned long long>(hi) << 32) | lo) >> (16 * halves));
+}
+
 }  // namespace fiery

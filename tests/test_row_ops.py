@@ -438,7 +438,7 @@ def test_entry_points_refuse(sim):
         with pytest.raises(bad):
             fwd(**kw)
     bwd = lambda ws=p, n=1 << 20, dx=p, dg=p, x_ld=8: sim.check(
-        d.fiery_layer_norm_bwd(p, 8, p, x_ld, 0, 2, 8, p, 0, p, p, dx, 8, dg, dg, ws, n, None))
+        d.fiery_layer_norm_bwd(p, 8, p, x_ld, 0, 1 << 20, 8, p, 0, p, p, dx, 8, dg, dg, ws, n, None))
     for kw in (dict(ws=None), dict(n=0), dict(dx=None, dg=None), dict(x_ld=-8)):
         with pytest.raises(bad):
             bwd(**kw)
