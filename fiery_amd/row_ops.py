@@ -156,30 +156,27 @@ def _norm_fwd(lib, x, weight, bias, eps, keep):
     rows, c = _sizes(x)
     xr, ld = _rows(x)
     y = _new(x)
+    stats = mean = rstd = None
     if keep:
         stats = torch.empty(2 * rows, dtype=torch.float32, device=x.device)        # mean, then rstd
         mean = stats.data_ptr()
         rstd = mean + 4 * rows
-    else:
-        stats = mean = rstd = None
     if rows:
         params = weight if weight is not None else bias
         _launch(lib, x, lib.dll.fiery_layer_norm_fwd, xr.data_ptr(), ld, _TYPES[x.dtype], rows, c, _ptr(weight), _ptr(bias),
                 0 if params is None else _TYPES[params.dtype], eps, y.data_ptr(), c, mean, rstd)
-    return y, xr, ld, stats
+    return y, xr, (rows, c, ld), stats
 
 
-def _param_grads(ctx, weight, bias, first, like):
-    """Buffers for the parameters' gradients where they are wanted: (dweight, dbias, type)."""
-    dw = _new(weight) if ctx.needs_input_grad[first] else None
-    db = torch.empty(bias[0], dtype=bias[1], device=like.device) if ctx.needs_input_grad[first + 1] else None
-    kind = weight.dtype if weight is not None else bias[1] if bias is not None else torch.float32
-    return dw, db, _TYPES[kind]
-
-
-def _workspace(lib, rows, c, like):
-    n = lib.dll.fiery_layer_norm_bwd_workspace_floats(rows, c)
-    return (torch.empty(n, dtype=torch.float32, device=like.device) if n else None), n
+def _param_grads(lib, weight, bias, want_w, want_b, rows, c, device):
+    """Buffers for the parameters' gradients where they are wanted, and the workspace of their sums: (dweight, dbias, their
+    FIERY_TYPE, workspace, its floats).  bias: its type or None.  The workspace is allocated per call: calls on other streams and
+    captured graphs share none."""
+    dw = _new(weight) if want_w else None
+    db = torch.empty(c, dtype=bias, device=device) if want_b else None
+    kind = weight.dtype if weight is not None else bias
+    n = lib.dll.fiery_layer_norm_bwd_workspace_floats(rows, c) if want_w or want_b else 0
+    return dw, db, 0 if kind is None else _TYPES[kind], torch.empty(n, dtype=torch.float32, device=device) if n else None, n
 
 
 class HipLayerNorm(torch.autograd.Function):
@@ -187,9 +184,9 @@ class HipLayerNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps, lib):
-        y, xr, ld, stats = _norm_fwd(lib, x, weight, bias, eps, True)
+        y, xr, sizes, stats = _norm_fwd(lib, x, weight, bias, eps, True)
         ctx.save_for_backward(xr, weight, stats)
-        ctx.meta = (ld, None if bias is None else (bias.shape, bias.dtype), lib)
+        ctx.meta = (sizes, None if bias is None else bias.dtype, lib)
         return y
 
     @staticmethod
@@ -199,18 +196,24 @@ class HipLayerNorm(torch.autograd.Function):
     @staticmethod
     def _grads(ctx, dy):
         xr, weight, stats = ctx.saved_tensors
-        ld, bias, lib = ctx.meta
-        rows, c = _sizes(xr)
-        dx = _new(xr) if ctx.needs_input_grad[0] else None
-        dw, db, kind = _param_grads(ctx, weight, bias, 1, xr)
-        if not rows:
-            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None, None
-        dr, dy_ld = _rows(dy)
-        ws, n = _workspace(lib, rows, c, xr) if dw is not None or db is not None else (None, 0)
-        mean = stats.data_ptr()
-        _launch(lib, xr, lib.dll.fiery_layer_norm_bwd, dr.data_ptr(), dy_ld, xr.data_ptr(), ld, _TYPES[xr.dtype], rows, c, _ptr(weight), kind,
-                mean, mean + 4 * rows, _ptr(dx), c, _ptr(dw), _ptr(db), _ptr(ws), n)
+        (rows, c, ld), bias, lib = ctx.meta
+        want_x, want_w, want_b, _, _ = ctx.needs_input_grad
+        dx = _new(xr) if want_x else None
+        dw, db, kind, ws, n = _param_grads(lib, weight, bias, want_w, want_b, rows, c, xr.device)
+        if rows:
+            dr, dy_ld = _rows(dy)
+            mean = stats.data_ptr()
+            _launch(lib, xr, lib.dll.fiery_layer_norm_bwd, dr.data_ptr(), dy_ld, xr.data_ptr(), ld, _TYPES[xr.dtype], rows, c, _ptr(weight), kind,
+                    mean, mean + 4 * rows, _ptr(dx), c, _ptr(dw), _ptr(db), _ptr(ws), n)
+        else:
+            _zero(dw, db)
         return dx, dw, db, None, None
+
+
+def _zero(*tensors):
+    for t in tensors:
+        if t is not None:
+            t.zero_()
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, *, lib=None):
@@ -300,7 +303,7 @@ def _join_fwd(lib, x, residual, weight, bias, mask, rng, call, eps, keep):
         _launch(lib, x, lib.dll.fiery_dropout_add_layer_norm_fwd, xr.data_ptr(), ld, _TYPES[x.dtype], rr.data_ptr(), r_ld, _TYPES[residual.dtype],
                 rows, c, _ptr(weight), _ptr(bias), 0 if params is None else _TYPES[params.dtype], eps, threshold, _ptr(rng) if threshold else None,
                 call, share, one, _ptr(used), y.data_ptr(), c, h.data_ptr(), c, mean, rstd)
-    return y, h, stats, used
+    return y, h, (rows, c), stats, used
 
 
 class HipDropoutAddLayerNorm(torch.autograd.Function):
@@ -308,10 +311,10 @@ class HipDropoutAddLayerNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, residual, weight, bias, mask, rng, call, eps, lib):
-        y, h, stats, used = _join_fwd(lib, x, residual, weight, bias, mask, rng, call, eps, True)
+        y, h, sizes, stats, used = _join_fwd(lib, x, residual, weight, bias, mask, rng, call, eps, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(h, weight, stats, used)
-        ctx.meta = (x.dtype, None if bias is None else (bias.shape, bias.dtype), mask, lib)
+        ctx.meta = (sizes, x.dtype, None if bias is None else bias.dtype, mask, lib)
         return y, h
 
     @staticmethod
@@ -321,26 +324,25 @@ class HipDropoutAddLayerNorm(torch.autograd.Function):
     @staticmethod
     def _grads(ctx, dy, dh):
         h, weight, stats, used = ctx.saved_tensors
-        dtype, bias, mask, lib = ctx.meta
-        rows, c = _sizes(h)
+        (rows, c), dtype, bias, mask, lib = ctx.meta
         threshold, share, one = mask
-        if dy is None:                                           # only h went on: no norm to differentiate
-            none = lambda i, like: None if not ctx.needs_input_grad[i] else torch.zeros(like[0], dtype=like[1], device=h.device)
-            dx = _dropout(lib, dh, None, dtype, mask, used, 0, None) if ctx.needs_input_grad[0] and dh is not None else None
-            return (dx, dh if ctx.needs_input_grad[1] else None, none(2, None if weight is None else (weight.shape, weight.dtype)), none(3, bias),
-                    None, None, None, None, None)
-        dx = _new(h, dtype) if ctx.needs_input_grad[0] else None
-        dr = _new(h) if ctx.needs_input_grad[1] else None
-        dw, db, kind = _param_grads(ctx, weight, bias, 2, h)
-        if not rows:
-            return dx, dr, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None, None, None, None, None
-        gr, dy_ld = _rows(dy)
-        hg, dh_ld = (None, 0) if dh is None else _rows(dh)
-        ws, n = _workspace(lib, rows, c, h) if dw is not None or db is not None else (None, 0)
-        mean = stats.data_ptr()
-        _launch(lib, h, lib.dll.fiery_dropout_add_layer_norm_bwd, gr.data_ptr(), dy_ld, _ptr(hg), dh_ld, h.data_ptr(), c, _TYPES[dtype],
-                _TYPES[h.dtype], rows, c, _ptr(weight), kind, mean, mean + 4 * rows, threshold, _ptr(used), share, one, _ptr(dx), c, _ptr(dr), c,
-                _ptr(dw), _ptr(db), _ptr(ws), n)
+        want_x, want_r, want_w, want_b = ctx.needs_input_grad[:4]
+        if dy is None:                                           # only h went on: there is no norm to differentiate
+            dw, db, _, _, _ = _param_grads(lib, weight, bias, want_w, want_b, 0, c, h.device)
+            _zero(dw, db)
+            dx = _dropout(lib, dh, None, dtype, mask, used, 0, None) if want_x and dh is not None else None
+            return dx, dh if want_r else None, dw, db, None, None, None, None, None
+        dx, dr = _new(h, dtype) if want_x else None, _new(h) if want_r else None
+        dw, db, kind, ws, n = _param_grads(lib, weight, bias, want_w, want_b, rows, c, h.device)
+        if rows:
+            gr, dy_ld = _rows(dy)
+            hg, dh_ld = (None, 0) if dh is None else _rows(dh)
+            mean = stats.data_ptr()
+            _launch(lib, h, lib.dll.fiery_dropout_add_layer_norm_bwd, gr.data_ptr(), dy_ld, _ptr(hg), dh_ld, h.data_ptr(), c, _TYPES[dtype],
+                    _TYPES[h.dtype], rows, c, _ptr(weight), kind, mean, mean + 4 * rows, threshold, _ptr(used), share, one, _ptr(dx), c, _ptr(dr), c,
+                    _ptr(dw), _ptr(db), _ptr(ws), n)
+        else:
+            _zero(dw, db)
         return dx, dr, dw, db, None, None, None, None, None
 
 

@@ -12,8 +12,8 @@ import torch
 ROOT = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 sys.path.insert(0, ROOT)
 
-SHAPES = [(1, 1), (5, 3), (3, 8), (4, 13), (2, 35), (3, 64), (2, 250), (2, 513), (2, 1030), (1, 2055), (2, 4099)]
-LONG = (1, 32773)
+SHAPES = [(1, 1), (5, 3), (3, 8), (4, 13), (2, 35), (3, 64), (2, 250), (2, 513), (2, 1030), (1, 2055), (1, 4099)]
+LONG = (1, 8197)
 TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
@@ -41,12 +41,12 @@ def main():
     torch.empty = empty
     done = 0
     for shape in SHAPES + [LONG]:
-        for dtype in TYPES if shape is not LONG else TYPES[:2]:
+        for dtype in TYPES if shape is not LONG else TYPES[1:2]:
             x, w, b = rows(shape, dtype), rows(shape[-1:], dtype), rows(shape[-1:], dtype)
             if case == 'norm':
                 y = row_ops.layer_norm(x, w, b, lib=lib)
                 torch.autograd.grad(y, (x, w, b), rows(shape, dtype).detach())
-            for per in ('element', 'channel', 'sample') if shape is not LONG else ('element',):
+            for per in ('element', 'channel', 'sample') if shape[-1] < 1000 else ('element',):
                 for stream in {dtype, torch.float32}:
                     r = rows(shape, stream)
                     if case == 'dropout':
