@@ -34,7 +34,7 @@ import os
 import torch
 import torch.nn.functional as F
 
-from . import native
+from . import native, row_ops
 from .backbone import mbconv_geometry, same_pads
 from .ops import Buf, ConvOp, identity_chan_map, round_up
 
@@ -112,6 +112,15 @@ TRAIN_WINOGRAD = os.environ.get('FIERY_TRAIN_WINOGRAD', '1') != '0'
 # sits 9.2e-4 from it instead of 3.9e-4, past that test's 2e-4 x scale bound, and a bound is not moved for 1 %.
 TRAIN_SPLIT = os.environ.get('FIERY_TRAIN_SPLIT', '1') != '0'
 TRAIN_SPLIT_FORWARD = os.environ.get('FIERY_TRAIN_SPLIT_FORWARD', '0') != '0'
+
+
+# How the image trunk's drop-connect draws its masks in training.  'torch' (the default): `torch.rand`, as efficientnet-pytorch does -
+# a run keeps the masks its torch seed always gave it.  'counter': the library's dropout (`row_ops.dropout`, per sample, the skip
+# added in the same launch; nothing of the mask is stored), numbered by `model.dropout_rng`.  `FIERY_TRAIN_DROP_CONNECT=counter`, or set
+# `train_graph.DROP_CONNECT` before the step.
+DROP_CONNECT = os.environ.get('FIERY_TRAIN_DROP_CONNECT', 'torch')
+if DROP_CONNECT not in ('torch', 'counter'):
+    raise ValueError(f"FIERY_TRAIN_DROP_CONNECT is 'torch' or 'counter', got {DROP_CONNECT!r}")
 
 
 def _train_forms():
@@ -578,6 +587,7 @@ def _counts_batches_once(method):
             return method(self, *args, **kwargs)
         finally:
             pending, self._counters = self._counters, None
+            self._advance_dropout()
             if pending:
                 torch._foreach_add_([t for t, _ in pending.values()], [k for _, k in pending.values()])
     return entry
@@ -592,6 +602,7 @@ class TrainGraph:
         self._conv = conv2d or HipConv2d.apply
         self._hip_ops = conv2d is None
         self._counters = None                         # {id: (num_batches_tracked, pending increments)} inside an entry point
+        self._dropouts = 0                            # dropouts of the pass so far: what numbers their masks
         self.whole_plane_pooling_as_means = True      # False: avg_pool3d + interpolate, operator for operator as the reference
         self.hip_trunk = os.environ.get('FIERY_HIP_TRUNK', '1') != '0'      # False: the image trunk + lift head as `Encoder.lift_head` (PyTorch-ROCm / MIOpen)
         if not self.hip_trunk:
@@ -654,6 +665,31 @@ class TrainGraph:
         return HipBatchNormAct.apply(x, norm.weight, norm.bias, norm.running_mean if (update or not batch_stats) else None,
                                      norm.running_var if (update or not batch_stats) else None, batch_stats, factor, norm.eps, relu,
                                      self.lib)
+
+    def dropout_add(self, x, skip, p, per):
+        """skip + dropout(x) of (N, C, H, W) tensors in one launch (`row_ops.dropout`): per 'channel' (`nn.Dropout2d`) or 'sample'
+        (drop-connect).  The masks are numbered by `model.dropout_rng` ([seed, call] on the device, made from torch's global seed
+        at its first use; set it to choose them) and the dropout's place in the pass; the pass advances the tensor when it ends,
+        so replays of a captured step draw new masks."""
+        if not self._hip_ops:                         # tests: a substituted convolution, any type or device
+            shape = (x.shape[0], x.shape[1], 1, 1) if per == 'channel' else (x.shape[0], 1, 1, 1)
+            return skip + x * F.dropout(x.new_ones(shape), p)
+        owner = self if self.m is None else self.m
+        rng = owner.__dict__.get('dropout_rng')
+        if rng is None or rng.device != x.device:
+            rng = row_ops.dropout_rng(int(torch.randint(1 << 62, (1,))), x.device) if rng is None else rng.to(x.device)
+            owner.__dict__['dropout_rng'] = rng
+        y = row_ops.dropout(x.float().permute(0, 2, 3, 1), p, rng, call=self._dropouts, per=per, residual=skip.float().permute(0, 2, 3, 1), lib=self.lib)
+        self._dropouts += 1
+        if self._counters is None:                    # a block on its own: no pass to number it in
+            self._advance_dropout()
+        return y.permute(0, 3, 1, 2)
+
+    def _advance_dropout(self):
+        if self._dropouts:
+            rng = (self if self.m is None else self.m).__dict__['dropout_rng']
+            rng[1:].add_(self._dropouts)
+            self._dropouts = 0
 
     def conv3d_frames(self, x, weight):
         """(B, C, T, H, W) x (Cout, Cin, kT, k, k) -> (B, Cout, T, H, W): `CausalConv3d`'s convolution (kT - 1 zero frames
@@ -742,13 +778,16 @@ class TrainGraph:
         return _frames_view(y, b, t, tm.receptive_field - 1)
 
     def bottleneck(self, x, blk):
-        """fiery/layers/convolutions.py:64-168 (Dropout2d(p=0) is the identity)."""
+        """fiery/layers/convolutions.py:64-168; its Dropout2d (p = 0 unless the caller sets it) drops channels of the branch while
+        training, in the launch that adds the skip."""
         L = blk.layers
+        p = L.dropout.p if L.dropout.training else 0.0
+        add = (lambda r, skip: r + skip) if p == 0.0 else (lambda r, skip: self.dropout_add(r, skip, p, 'channel'))
         r = self.bn_act(self.conv2d(x, L.conv_down_project), L.abn_down_project[0], relu=True)
         r = self.bn_act(self.conv2d(r, L.conv), L.abn[0], relu=True)
         r = self.bn_act(self.conv2d(r, L.conv_up_project), L.abn_up_project[0], relu=True)
         if blk.projection is None:
-            return r + x
+            return add(r, x)
         skip = x
         if blk.downsample:
             # odd sizes are padded first so that the pooled skip meets the strided convolution's size (convolutions.py:160-162)
@@ -757,7 +796,7 @@ class TrainGraph:
             else:
                 skip = F.max_pool2d(F.pad(skip, (0, skip.shape[-1] % 2, 0, skip.shape[-2] % 2), value=0), 2, 2)
         skip = self.bn_act(self.conv2d(skip, blk.projection.conv_skip_proj), blk.projection.bn_skip_proj, relu=False)
-        return r + skip
+        return add(r, skip)
 
     def gru_cell(self, x, state, gru):
         """fiery/layers/temporal.py:49-62 (note (1 - reset) * state)."""
@@ -982,6 +1021,8 @@ class TrainGraph:
         x = self.bn_act(self._same_pad_conv(x, blk._project_conv), blk._bn2, relu=False)
         if stride == 1 and cin == cout:
             if drop_connect_rate and blk.training:
+                if DROP_CONNECT == 'counter':
+                    return self.dropout_add(x, inputs, drop_connect_rate, 'sample')
                 keep = 1.0 - drop_connect_rate
                 mask = torch.floor(keep + torch.rand(x.shape[0], 1, 1, 1, dtype=x.dtype, device=x.device))
                 x = x / keep * mask

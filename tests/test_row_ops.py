@@ -464,3 +464,145 @@ def test_row_kernels_stay_inside_their_operands(sim, case, where):
     res = subprocess.run([sys.executable, os.path.join(root, 'tests', 'sim', 'guard_rows.py'), case, where], cwd=root, capture_output=True, text=True,
                          timeout=900)
     assert res.returncode == 0 and f'ok {case} {where} (' in res.stdout, res.stdout[-1500:] + res.stderr[-3000:]
+
+
+# ---- together, captured, on other streams, past 32 bits ------------------------------------------------------------------------------------
+def _block(x, w1, b1, w2, b2, rng, lib=None):
+    """A residual block as a model uses the operators: norm, branch, channel dropout + skip, then the joined norm of a second branch."""
+    branch = torch.relu(row_ops.layer_norm(x, w1, b1, lib=lib))
+    skip = row_ops.dropout(branch, 0.2, rng, call=0, per='channel', residual=x, lib=lib)
+    return row_ops.dropout_add_layer_norm(torch.tanh(skip), skip, w2, b2, 0.3, rng, call=1, lib=lib)
+
+
+def _block_leaves(device, shape, seed=50):
+    c = shape[-1]
+    return [make(shape, F32, device, seed).requires_grad_()] + [make((c,), F32, device, seed + 1 + i, 0.2, 1.0 if i % 2 == 0 else 0.0).requires_grad_() for i in range(4)]
+
+
+def test_operators_together_against_64_bit_autograd(on):
+    """Outputs and gradients of the chain against torch's autograd of its 64-bit definition.  Errors of single operators stay below
+    40 u of a row's largest value here (rows of 24: DEPTH / 2 + 6 is 33); four in a row with factors up to 3 each (norms of
+    spread 1, weights up to 1.6, scales up to 1.43): 4 * 40 * 3^3 u = 2.6e-4 of the tensor's largest value."""
+    shape = (3, 5, 24)
+    leaves, rng = _block_leaves(on.device, shape), row_ops.dropout_rng(31, on.device)
+    y, h = _block(*leaves, rng, lib=on.lib)
+    gy, gh = make(shape, F32, on.device, 60), make(shape, F32, on.device, 61)
+    got = [y, h, *torch.autograd.grad((y, h), leaves, (gy, gh))]
+    x, w1, b1, w2, b2 = ref = [t.detach().double().cpu().requires_grad_() for t in leaves]
+    m1, m2 = kept(shape, 0.2, 31, 0, 'channel'), kept(shape, 0.3, 31, 1, 'element')
+    norm = lambda t, w, b: norm64(t, None, None, 1e-5)[2] * w + b
+    skip = x + torch.relu(norm(x, w1, b1)) * m1
+    h64 = skip + torch.tanh(skip) * m2
+    y64 = norm(h64, w2, b2)
+    want = [y64, h64, *torch.autograd.grad((y64, h64), ref, (gy.double().cpu(), gh.double().cpu()))]
+    for g, t in zip(got, want):
+        assert (g.detach().double().cpu() - t.detach()).abs().max() <= 4 * 40 * 27 * U * t.abs().max()
+
+
+@pytest.mark.gpu
+def test_captured_step_draws_new_masks_at_every_replay(hip):
+    """Forward, backward and the advance of the numbers in one hipGraph; every replay equals the eager step of its numbers bit for
+    bit, with eager work of the same operators in between."""
+    shape = (4, 300, 64)
+    x0 = make(shape, F32, 'cuda', 70)
+    gy = make(shape, F32, 'cuda', 71)
+
+    def step(x, params, rng):
+        leaves = [x.detach().requires_grad_()] + [p.detach().requires_grad_() for p in params]
+        y, h = _block(*leaves, rng)
+        grads = torch.autograd.grad((y, h), leaves, (gy, gy))
+        rng[1:].add_(2)
+        return [y.detach(), h.detach(), *grads]
+    params = [t.detach() for t in _block_leaves('cuda', shape)[1:]]
+    rng, eager = row_ops.dropout_rng(8, 'cuda'), row_ops.dropout_rng(8, 'cuda')
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(x0, params, rng)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(x0, params, rng)
+    eager[1] += 4
+    assert torch.equal(rng, eager)                       # the warm-up's two steps; the capture itself ran nothing
+    first = None
+    for k in range(3):
+        graph.replay()
+        want = step(x0, params, eager)
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b), k
+        assert torch.equal(rng, eager)
+        if first is None:
+            first = out[0].clone()
+    assert not torch.equal(first, out[0])
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(hip):
+    """The same step on two side streams without a wait between them: nothing is shared (workspaces are allocated per call)."""
+    shape = (6, 700, 200)
+    want, streams, got = [], [torch.cuda.Stream() for _ in range(2)], []
+    leaves = [_block_leaves('cuda', shape, 80 + 10 * i) for i in range(2)]
+    rng = row_ops.dropout_rng(2, 'cuda')
+    gy = make(shape, F32, 'cuda', 99)
+    for i in range(2):
+        y, h = _block(*leaves[i], rng)
+        want.append([y, h, *torch.autograd.grad((y, h), leaves[i], (gy, gy))])
+    torch.cuda.synchronize()
+    for i, s in enumerate(streams):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            y, h = _block(*leaves[i], rng)
+            got.append([y, h, *torch.autograd.grad((y, h), leaves[i], (gy, gy))])
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(hip):
+    """Over 2^31 elements, and rows 1.2e9 elements apart: the rows at the far end are those of a small call."""
+    c, rows = 4104, (1 << 31) // 4104 + 7
+    x = torch.empty(rows, c, dtype=BF16, device='cuda').normal_(generator=torch.Generator(device='cuda').manual_seed(1)).requires_grad_()
+    w = make((c,), F32, 'cuda', 90, 0.2, 1.0).requires_grad_()
+    y = row_ops.layer_norm(x, w)
+    assert torch.equal(y[-9:], row_ops.layer_norm(x[-9:], w)) and torch.equal(y[:9], row_ops.layer_norm(x[:9], w))
+    dx, = torch.autograd.grad(y, x, x.detach())
+    tail = x.detach()[-9:].requires_grad_()
+    assert torch.equal(dx[-9:], torch.autograd.grad(row_ops.layer_norm(tail, w), tail, tail.detach())[0])
+    del y, dx
+    rng = row_ops.dropout_rng(4, 'cuda')
+    d = row_ops.dropout(x.detach(), 0.5, rng)
+    words = [h for unit in range(c // 8) for v in philox([unit, rows - 1, 0, 0], [4, 0]) for h in (v & 0xffff, v >> 16)]
+    keep = torch.tensor(words, device='cuda') >= 32768
+    assert torch.equal(d[-1], torch.where(keep, x.detach()[-1] * 2, torch.zeros_like(d[-1])))
+    del d, x
+    far = torch.zeros(2 * 1_200_000_000 + 40, dtype=F16, device='cuda').as_strided((3, 40), (1_200_000_000, 1))
+    far.copy_(make((3, 40), F16, 'cuda', 91))
+    assert row_ops._rows(far)[1] == 1_200_000_000
+    assert torch.equal(row_ops.layer_norm(far), row_ops.layer_norm(far.contiguous()))
+    assert torch.equal(row_ops.dropout(far, 0.3, rng, residual=far), row_ops.dropout(far.contiguous(), 0.3, rng, residual=far.contiguous()))
+
+
+def test_calls_go_to_the_tensors_device_and_stream(monkeypatch):
+    """A tensor on another device than the current one: the launch happens with that device current and on its stream."""
+    seen = []
+
+    class Guard:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            seen.append(('enter', self.dev))
+
+        def __exit__(self, *a):
+            seen.append(('exit', self.dev))
+    monkeypatch.setattr(torch.cuda, 'device', Guard)
+    monkeypatch.setattr(torch._C, '_cuda_getDevice', lambda: 0, raising=False)
+    monkeypatch.setattr(torch._C, '_cuda_getCurrentRawStream', lambda dev: 1000 + dev, raising=False)
+    entry = lambda *args: seen.append(args) or 0
+    for dev in (0, 1):
+        row_ops._launch(None, type('T', (), dict(get_device=lambda self, d=dev: d))(), entry, 'a')
+    assert seen == [('a', 1000), ('enter', 1), ('a', 1001), ('exit', 1)]
