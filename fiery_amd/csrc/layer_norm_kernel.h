@@ -505,16 +505,30 @@ inline int even_blocks(int64_t passes, int64_t most) {
     const int64_t rounds = (passes + most - 1) / most;
     return static_cast<int>((passes + rounds - 1) / rounds);
 }
-// workgroups of the backward pass = partial rows of dgamma / dbeta
-inline int norm_bwd_blocks(int64_t rows, int C) {
+// Workgroups per CU.  More of them than it takes to keep memory busy cost: the streams' pages are spread wider (forward, 64 fp32
+// columns: 44 us with 2, 48 with 8 for 480,000 rows), and every workgroup of the backward pass leaves a partial row (4096 bf16
+// columns, 8192 rows: 44 us with 1, 55 with 4).  Forward: 512 lanes with 32 bytes or 1024 with 16 (4096 bf16 columns: 36 us with
+// 1 workgroup, 24 with 4); ragged widths, which are bound by their arithmetic, twice that.  Backward, whose next row is on its
+// way already: 16 KB of each tensor in flight where wavefronts hold the rows (bf16, 64 columns: 73 us with 1, 39 with 4, 44 with 8), 8 KB
+// where workgroups do.
+inline int norm_fwd_per_cu(const NormShape& s, int C, int unit_bytes) {
+    const int n = (C % kUnit ? 2 : 1) * 16384 / unit_bytes / s.block();
+    return n < 2 ? 2 : n;
+}
+inline int norm_bwd_per_cu(const NormShape& s, int unit_bytes) {
+    const int n = (s.threads ? 8192 : 16384) / (s.block() * s.nv * unit_bytes);
+    return n < 1 ? 1 : n;
+}
+// workgroups of the backward pass = partial rows of dgamma / dbeta; unit_bytes: of the wider of the tensors (the largest for a workspace)
+inline int norm_bwd_blocks(int64_t rows, int C, int unit_bytes) {
     const NormShape s = norm_shape(C);
     if (s.nv == 0) return static_cast<int>(rows < 16 ? rows : 16);
     const int64_t passes = (rows + s.per_block() - 1) / s.per_block();
     if (passes <= 4) return 1;                                               // one workgroup writes the results itself
-    return even_blocks(passes, static_cast<int64_t>(row_ops_cus()) * (s.threads ? (s.threads < 512 ? 512 / s.threads : 1) : 4));
+    return even_blocks(passes, static_cast<int64_t>(row_ops_cus()) * norm_bwd_per_cu(s, unit_bytes));
 }
 inline int64_t norm_bwd_workspace_floats(int64_t rows, int C) {
-    const int blocks = norm_bwd_blocks(rows, C);
+    const int blocks = norm_bwd_blocks(rows, C, 16);
     if (blocks == 1 && norm_shape(C).nv) return 0;
     return static_cast<int64_t>(blocks) * 2 * ((C + kUnit - 1) / kUnit * kUnit);
 }
@@ -537,8 +551,8 @@ void norm_fwd_launch(NormFwdArgs a, hipStream_t stream) {
     const NormShape s = norm_shape(a.C);
     a.lane_bits = s.lane_bits;
     const int64_t passes = (static_cast<int64_t>(a.rows) + s.per_block() - 1) / s.per_block();
-    // as many workgroups as are resident at once: the parameters are read once per workgroup
-    const dim3 grid(even_blocks(passes, static_cast<int64_t>(row_ops_cus()) * (2048 / s.block()))), block(s.block());
+    const int per_cu = norm_fwd_per_cu(s, a.C, kUnit * sizeof(typename S::store));
+    const dim3 grid(even_blocks(passes, static_cast<int64_t>(row_ops_cus()) * per_cu)), block(s.block());
     const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a); };
     if (s.nv == 0)
         run(k_norm_fwd_long<T, S, JOIN>);
@@ -561,7 +575,7 @@ void norm_bwd_launch(NormBwdArgs a, hipStream_t stream) {
     const NormShape s = norm_shape(a.C);
     a.lane_bits = s.lane_bits;
     const bool sums = a.dgamma || a.dbeta;
-    const int blocks = norm_bwd_blocks(a.rows, a.C);
+    const int blocks = norm_bwd_blocks(a.rows, a.C, kUnit * sizeof(typename S::store));
     if (!sums) a.partial = nullptr;
     if (s.nv == 0) {
         const int units = (a.C + kUnit - 1) / kUnit, most = 2 * row_ops_cus();

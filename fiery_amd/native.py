@@ -310,6 +310,7 @@ class Lib:
         for name, (restype, argtypes) in _SIGNATURES.items():
             fn = getattr(self.dll, name)          # AttributeError here = symbol missing from the build
             fn.restype, fn.argtypes = restype, argtypes
+        self.launches_on_gpu = hasattr(self.dll, 'hipLaunchKernel')       # (False: the CPU simulator's build of the sources)
         self.dll = _EntryPoints(self.dll)
         got = self.dll.fiery_abi_version()
         if got != ABI_VERSION:

@@ -60,11 +60,9 @@ def _sizes(x):
 
 
 def _lib_for(lib, x):
-    if lib is not None:
-        return lib
-    if not x.is_cuda:
+    if not x.is_cuda and (lib is None or lib.launches_on_gpu):   # (a host address in a GPU kernel faults)
         raise ValueError('row operators run on the GPU: x is on ' + str(x.device))
-    return native.get()
+    return native.get() if lib is None else lib
 
 
 def _launch(lib, x, entry, *args):
@@ -96,6 +94,8 @@ def _check_x(x, what):
         raise ValueError(f'{what}: x is a float32, bfloat16 or float16 tensor, got {getattr(x, "dtype", type(x).__name__)}')
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError(f'{what}: the last axis of x has no values: shape {tuple(x.shape)}')
+    if x.shape[-1] > 1 << 30 or x.numel() // x.shape[-1] >= 1 << 31:
+        raise ValueError(f'{what}: at most 2^30 columns and 2^31 - 1 rows, got shape {tuple(x.shape)}')
 
 
 def _check_params(x, weight, bias, what):

@@ -422,6 +422,16 @@ def test_refusals(sim):
             call()
     with pytest.raises(ValueError, match='GPU'):
         row_ops.layer_norm(x)                                      # host tensors without a library of their own
+    product = type('Lib', (), dict(launches_on_gpu=True))()
+    for call in (lambda: row_ops.layer_norm(x, lib=product), lambda: row_ops.dropout(x, 0.5, rng, lib=product),
+                 lambda: row_ops.dropout_add_layer_norm(x, x, p=0.5, rng=rng, lib=product)):
+        with pytest.raises(ValueError, match='GPU'):                # host addresses never reach the GPU's library
+            call()
+    huge = torch.zeros(1, dtype=torch.float16)
+    for shape in ((1, (1 << 32) + 5), (1 << 31, 2)):                # (a width that a 32-bit argument would cut to 5)
+        for call in (norm, lambda t: drop(t, 0.5, rng), lambda t: join(t, t)):
+            with pytest.raises(ValueError, match='columns'):
+                call(huge.expand(shape))
     y = norm(x.clone().requires_grad_())
     with pytest.raises(RuntimeError):                               # gradients of gradients
         g, = torch.autograd.grad(y.sum(), y.grad_fn.next_functions[0][0].variable, create_graph=True)
