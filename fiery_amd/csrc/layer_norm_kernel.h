@@ -92,40 +92,40 @@ __device__ __forceinline__ float rstd_of(float x) {
 }
 
 // one unit of h: x alone, or residual + drop(x), written out as it is read
-template <typename T, typename S, bool JOIN, bool RAGGED>
-__device__ __forceinline__ void load_h(const NormFwdArgs& a, const DropKey& key, long long row, int unit, int count, bool write, float (&v)[kUnit]) {
+template <typename T, typename S, bool JOIN, int RAGGED>
+__device__ __forceinline__ void load_h(const NormFwdArgs& a, const DropKey& key, long long row, bool live, int unit, int count, bool write, float (&v)[kUnit]) {
     const long long c = static_cast<long long>(unit) * kUnit;
-    const Raw<T> x = load_raw<T, RAGGED>(static_cast<const typename T::store*>(a.x) + row * a.x_ld + c, count, a.C);
+    const Raw<T> x = load_raw<T, RAGGED>(static_cast<const typename T::store*>(a.x) + row * a.x_ld + c, live, count, a.C);
     if constexpr (!JOIN) {
         unpack<T, RAGGED>(x, count, a.C, v);
     } else {
-        const Raw<S> residual = load_raw<S, RAGGED>(static_cast<const typename S::store*>(a.residual) + row * a.res_ld + c, count, a.C);
+        const Raw<S> residual = load_raw<S, RAGGED>(static_cast<const typename S::store*>(a.residual) + row * a.res_ld + c, live, count, a.C);
         float r[kUnit];
         unpack<T, RAGGED>(x, count, a.C, v);
         unpack<S, RAGGED>(residual, count, a.C, r);
         drop_unit(a.drop, key, static_cast<unsigned>(row), static_cast<unsigned>(unit), v);
 #pragma unroll
         for (int j = 0; j < kUnit; ++j) v[j] += r[j];
-        if (write) store_unit<S, RAGGED>(static_cast<typename S::store*>(a.h) + row * a.h_ld + c, count, v);
+        if (write && live) store_unit<S, RAGGED>(static_cast<typename S::store*>(a.h) + row * a.h_ld + c, count, v);
     }
 }
 
-template <bool RAGGED>
+template <int RAGGED>
 __device__ __forceinline__ void distances(const float (&v)[kUnit], int count, float mean, float& q) {
-    if constexpr (RAGGED) {
+    if (RAGGED == 1 || (RAGGED == 2 && count < kUnit)) {
 #pragma unroll
         for (int j = 0; j < kUnit; ++j) {
             const float d = j < count ? v[j] - mean : 0.f;
             q += d * d;
         }
-    } else {
+    } else if (count) {
         float p = 0.f;
 #pragma unroll
         for (int j = 0; j < kUnit; ++j) {
             const float d = v[j] - mean;
             p += d * d;
         }
-        q += count ? p : 0.f;
+        q += p;
     }
 }
 template <typename S>
@@ -135,7 +135,7 @@ __device__ __forceinline__ void sum_stored(const float (&v)[kUnit], float& s) {
 #pragma unroll
     for (int j = 0; j < kUnit; ++j) s += r[j];
 }
-template <typename T, typename S, bool JOIN, int NV, int THREADS, bool RAGGED>
+template <typename T, typename S, bool JOIN, int NV, int THREADS, int RAGGED>
 __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_fwd(NormFwdArgs a) {
     __shared__ float slots[2][2][16];
     int turn = 0;
@@ -149,11 +149,13 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_fwd(NormFwdArg
         drop_note(a.drop);
     }
     float ga[NV][kUnit], be[NV][kUnit];
+    int count[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int unit = i * lanes + sub, count = unit_count<RAGGED>(a.C, unit);
-        load_typed(a.gamma, a.param_type, static_cast<long long>(unit) * kUnit, count, a.C, 1.f, ga[i]);
-        load_typed(a.beta, a.param_type, static_cast<long long>(unit) * kUnit, count, a.C, 0.f, be[i]);
+        const int unit = i * lanes + sub;
+        count[i] = unit_count<RAGGED>(a.C, unit);
+        load_typed<RAGGED>(a.gamma, a.param_type, static_cast<long long>(unit) * kUnit, count[i], a.C, 1.f, ga[i]);
+        load_typed<RAGGED>(a.beta, a.param_type, static_cast<long long>(unit) * kUnit, count[i], a.C, 0.f, be[i]);
     }
     // (every lane of a wavefront walks the loop as often as its neighbours: the exchanges need all of them)
     for (long long first = static_cast<long long>(blockIdx.x) * per_block; first < a.rows; first += static_cast<long long>(gridDim.x) * per_block) {
@@ -161,13 +163,10 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_fwd(NormFwdArg
         const bool live = row < a.rows;
         constexpr bool two = JOIN && sizeof(typename S::store) == 2;            // the stored h has statistics of its own
         float v[NV][kUnit];
-        int count[NV];
         float s[two ? 2 : 1] = {}, q[two ? 2 : 1] = {};
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int unit = i * lanes + sub;
-            count[i] = live ? unit_count<RAGGED>(a.C, unit) : 0;
-            load_h<T, S, JOIN, RAGGED>(a, key, row, unit, count[i], true, v[i]);
+            load_h<T, S, JOIN, RAGGED>(a, key, row, live, i * lanes + sub, count[i], true, v[i]);
 #pragma unroll
             for (int j = 0; j < kUnit; ++j) s[0] += v[i][j];
             if constexpr (two) sum_stored<S>(v[i], s[1]);
@@ -194,7 +193,7 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_fwd(NormFwdArg
             float out[kUnit];
 #pragma unroll
             for (int j = 0; j < kUnit; ++j) out[j] = (v[i][j] - mean) * rstd * ga[i][j] + be[i][j];
-            store_unit<T, RAGGED>(static_cast<typename T::store*>(a.y) + row * a.y_ld + static_cast<long long>(i * lanes + sub) * kUnit, count[i], out);
+            if (live) store_unit<T, RAGGED>(static_cast<typename T::store*>(a.y) + row * a.y_ld + static_cast<long long>(i * lanes + sub) * kUnit, count[i], out);
         }
     }
 }
@@ -215,7 +214,7 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_long(NormFwdArgs a) {
         constexpr bool two = JOIN && sizeof(typename S::store) == 2;
         float v[kUnit], s[two ? 2 : 1] = {}, q[two ? 2 : 1] = {};
         for (int u = threadIdx.x; u < units; u += blockDim.x) {
-            load_h<T, S, JOIN, true>(a, key, row, u, unit_count<true>(a.C, u), true, v);
+            load_h<T, S, JOIN, 2>(a, key, row, true, u, unit_count<2>(a.C, u), true, v);
 #pragma unroll
             for (int j = 0; j < kUnit; ++j) s[0] += v[j];
             if constexpr (two) sum_stored<S>(v, s[1]);
@@ -223,13 +222,13 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_long(NormFwdArgs a) {
         row_sums<1024>(s, 64, slots, turn);
         const float mean = mean_of(s[0], a.C, a.inv_c);
         for (int u = threadIdx.x; u < units; u += blockDim.x) {
-            const int count = unit_count<true>(a.C, u);
-            load_h<T, S, JOIN, true>(a, key, row, u, count, false, v);
-            distances<true>(v, count, mean, q[0]);
+            const int count = unit_count<2>(a.C, u);
+            load_h<T, S, JOIN, 2>(a, key, row, true, u, count, false, v);
+            distances<2>(v, count, mean, q[0]);
             if constexpr (two) {
                 float r[kUnit];
                 as_stored<S>(v, r);
-                distances<true>(r, count, mean_of(s[1], a.C, a.inv_c), q[1]);
+                distances<2>(r, count, mean_of(s[1], a.C, a.inv_c), q[1]);
             }
         }
         row_sums<1024>(q, 64, slots, turn);
@@ -239,20 +238,20 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_long(NormFwdArgs a) {
             a.rstd[row] = two ? rstd_of(q[two ? 1 : 0] * a.inv_c + a.eps) : rstd;
         }
         for (int u = threadIdx.x; u < units; u += blockDim.x) {
-            const int count = unit_count<true>(a.C, u);
-            load_h<T, S, JOIN, true>(a, key, row, u, count, false, v);
+            const int count = unit_count<2>(a.C, u);
+            load_h<T, S, JOIN, 2>(a, key, row, true, u, count, false, v);
             float ga[kUnit], be[kUnit];
-            load_typed(a.gamma, a.param_type, static_cast<long long>(u) * kUnit, count, a.C, 1.f, ga);
-            load_typed(a.beta, a.param_type, static_cast<long long>(u) * kUnit, count, a.C, 0.f, be);
+            load_typed<2>(a.gamma, a.param_type, static_cast<long long>(u) * kUnit, count, a.C, 1.f, ga);
+            load_typed<2>(a.beta, a.param_type, static_cast<long long>(u) * kUnit, count, a.C, 0.f, be);
 #pragma unroll
             for (int j = 0; j < kUnit; ++j) v[j] = (v[j] - mean) * rstd * ga[j] + be[j];
-            store_unit<T, true>(static_cast<typename T::store*>(a.y) + row * a.y_ld + static_cast<long long>(u) * kUnit, count, v);
+            store_unit<T, 2>(static_cast<typename T::store*>(a.y) + row * a.y_ld + static_cast<long long>(u) * kUnit, count, v);
         }
     }
 }
 
 // One unit of the backward pass's results from its dy (gg = dy gamma), xhat and the row's sums.
-template <typename T, typename S, bool JOIN, bool RAGGED>
+template <typename T, typename S, bool JOIN, int RAGGED>
 __device__ __forceinline__ void store_grads(const NormBwdArgs& a, const DropKey& key, long long row, int unit, int count, const float (&gg)[kUnit],
                                             const float (&xhat)[kUnit], const Raw<S>& dh, float rstd, float m1, float m2) {
     const long long c = static_cast<long long>(unit) * kUnit;
@@ -275,7 +274,7 @@ __device__ __forceinline__ void store_grads(const NormBwdArgs& a, const DropKey&
     store_unit<T, RAGGED>(static_cast<typename T::store*>(a.dx) + row * a.dx_ld + c, count, out);
 }
 
-template <typename T, typename S, bool JOIN, int NV, int THREADS, bool RAGGED>
+template <typename T, typename S, bool JOIN, int NV, int THREADS, int RAGGED>
 __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_bwd(NormBwdArgs a) {
     typedef typename std::conditional<JOIN, S, T>::type H;
     __shared__ float slots[2][2][16];
@@ -288,9 +287,11 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_bwd(NormBwdArg
     if constexpr (JOIN)
         if (a.drop.threshold) key = drop_key(a.drop);
     float ga[NV][kUnit], dg[NV][kUnit], db[NV][kUnit];
+    int count[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        load_typed(a.gamma, a.param_type, static_cast<long long>(i * lanes + sub) * kUnit, unit_count<RAGGED>(a.C, i * lanes + sub), a.C, 1.f, ga[i]);
+        count[i] = unit_count<RAGGED>(a.C, i * lanes + sub);
+        load_typed<RAGGED>(a.gamma, a.param_type, static_cast<long long>(i * lanes + sub) * kUnit, count[i], a.C, 1.f, ga[i]);
 #pragma unroll
         for (int j = 0; j < kUnit; ++j) dg[i][j] = db[i][j] = 0.f;
     }
@@ -306,10 +307,10 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_bwd(NormBwdArg
         const long long at = live ? row : 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int unit = i * lanes + sub, count = live ? unit_count<RAGGED>(a.C, unit) : 0;
-            h_next[i] = load_raw<H, RAGGED>(static_cast<const typename H::store*>(a.h) + at * a.h_ld + static_cast<long long>(unit) * kUnit, count, a.C);
-            g_next[i] = load_raw<T, RAGGED>(static_cast<const typename T::store*>(a.dy) + at * a.dy_ld + static_cast<long long>(unit) * kUnit, count, a.C);
-            if (JOIN && a.dh) d_next[i] = load_raw<S, RAGGED>(static_cast<const typename S::store*>(a.dh) + at * a.dh_ld + static_cast<long long>(unit) * kUnit, count, a.C);
+            const int unit = i * lanes + sub;
+            h_next[i] = load_raw<H, RAGGED>(static_cast<const typename H::store*>(a.h) + at * a.h_ld + static_cast<long long>(unit) * kUnit, live, count[i], a.C);
+            g_next[i] = load_raw<T, RAGGED>(static_cast<const typename T::store*>(a.dy) + at * a.dy_ld + static_cast<long long>(unit) * kUnit, live, count[i], a.C);
+            if (JOIN && a.dh) d_next[i] = load_raw<S, RAGGED>(static_cast<const typename S::store*>(a.dh) + at * a.dh_ld + static_cast<long long>(unit) * kUnit, live, count[i], a.C);
         }
         mean_next = live ? a.mean[row] : 0.f;                                      // (a row that is none has xhat 0, whatever row 0 holds)
         rstd_next = live ? a.rstd[row] : 0.f;
@@ -323,10 +324,8 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_bwd(NormBwdArg
         const float mean = mean_next, rstd = rstd_next;
         float gg[NV][kUnit], xhat[NV][kUnit], s[2] = {0.f, 0.f};
         Raw<S> dh[NV];
-        int count[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            count[i] = live ? unit_count<RAGGED>(a.C, i * lanes + sub) : 0;
             dh[i] = d_next[i];
             unpack<H, RAGGED>(h_next[i], count[i], a.C, xhat[i]);
             unpack<T, RAGGED>(g_next[i], count[i], a.C, gg[i]);
@@ -347,7 +346,7 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_bwd(NormBwdArg
         const float m1 = s[0] * a.inv_c, m2 = s[1] * a.inv_c;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (count[i]) store_grads<T, S, JOIN, RAGGED>(a, key, at, i * lanes + sub, count[i], gg[i], xhat[i], dh[i], rstd, m1, m2);
+            if (live && count[i]) store_grads<T, S, JOIN, RAGGED>(a, key, at, i * lanes + sub, count[i], gg[i], xhat[i], dh[i], rstd, m1, m2);
     }
     if (!a.partial && !a.dgamma && !a.dbeta) return;
     const int width = (a.C + kUnit - 1) / kUnit * kUnit;
@@ -418,12 +417,12 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormBwdArgs a) {
         for (int walk = 0; walk < 2; ++walk) {
             const float m1 = s[0] * a.inv_c, m2 = s[1] * a.inv_c;
             for (int u = threadIdx.x; u < units; u += blockDim.x) {
-                const int count = unit_count<true>(a.C, u);
+                const int count = unit_count<2>(a.C, u);
                 const long long c = static_cast<long long>(u) * kUnit;
-                load_unit<H, true>(static_cast<const typename H::store*>(a.h) + row * a.h_ld + c, count, a.C, xhat);
-                load_unit<T, true>(static_cast<const typename T::store*>(a.dy) + row * a.dy_ld + c, count, a.C, gg);
+                load_unit<H, 2>(static_cast<const typename H::store*>(a.h) + row * a.h_ld + c, count, a.C, xhat);
+                load_unit<T, 2>(static_cast<const typename T::store*>(a.dy) + row * a.dy_ld + c, count, a.C, gg);
                 float ga[kUnit];
-                load_typed(a.gamma, a.param_type, c, count, a.C, 1.f, ga);
+                load_typed<2>(a.gamma, a.param_type, c, count, a.C, 1.f, ga);
 #pragma unroll
                 for (int j = 0; j < kUnit; ++j) {
                     xhat[j] = (xhat[j] - mean) * rstd;
@@ -437,8 +436,8 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormBwdArgs a) {
                     }
                 } else {
                     Raw<S> dh = {};
-                    if (JOIN && a.dh) dh = load_raw<S, true>(static_cast<const typename S::store*>(a.dh) + row * a.dh_ld + c, count, a.C);
-                    store_grads<T, S, JOIN, true>(a, key, row, u, count, gg, xhat, dh, rstd, m1, m2);
+                    if (JOIN && a.dh) dh = load_raw<S, 2>(static_cast<const typename S::store*>(a.dh) + row * a.dh_ld + c, true, count, a.C);
+                    store_grads<T, S, JOIN, 2>(a, key, row, u, count, gg, xhat, dh, rstd, m1, m2);
                 }
             }
             if (walk == 0) row_sums<1024>(s, 64, slots, turn);
@@ -449,14 +448,14 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormBwdArgs a) {
 // dgamma, dbeta of one unit of columns over the strip blockIdx.y of the rows, one partial row per strip
 template <typename T, typename H>
 __global__ __launch_bounds__(256) void k_norm_bwd_cols_long(NormBwdArgs a) {
-    const int unit = blockIdx.x * 256 + threadIdx.x, count = unit_count<true>(a.C, unit);
+    const int unit = blockIdx.x * 256 + threadIdx.x, count = unit_count<2>(a.C, unit);
     if (count == 0) return;
     const int width = (a.C + kUnit - 1) / kUnit * kUnit;
     const long long c = static_cast<long long>(unit) * kUnit;
     float dg[kUnit] = {}, db[kUnit] = {}, h[kUnit], g[kUnit];
     for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
-        load_unit<H, true>(static_cast<const typename H::store*>(a.h) + row * a.h_ld + c, count, a.C, h);
-        load_unit<T, true>(static_cast<const typename T::store*>(a.dy) + row * a.dy_ld + c, count, a.C, g);
+        load_unit<H, 2>(static_cast<const typename H::store*>(a.h) + row * a.h_ld + c, count, a.C, h);
+        load_unit<T, 2>(static_cast<const typename T::store*>(a.dy) + row * a.dy_ld + c, count, a.C, g);
         const float mean = a.mean[row], rstd = a.rstd[row];
 #pragma unroll
         for (int j = 0; j < kUnit; ++j) {
@@ -515,17 +514,20 @@ inline int norm_fwd_per_cu(const NormShape& s, int C, int unit_bytes) {
     const int n = (C % kUnit ? 2 : 1) * 16384 / unit_bytes / s.block();
     return n < 2 ? 2 : n;
 }
-inline int norm_bwd_per_cu(const NormShape& s, int unit_bytes) {
-    const int n = (s.threads ? 8192 : 16384) / (s.block() * s.nv * unit_bytes);
+inline int norm_bwd_per_cu(const NormShape& s, int C, int unit_bytes) {
+    const int n = (C % kUnit && s.threads ? 2 : 1) * (s.threads ? 8192 : 16384) / (s.block() * s.nv * unit_bytes);
     return n < 1 ? 1 : n;
 }
 // workgroups of the backward pass = partial rows of dgamma / dbeta; unit_bytes: of the wider of the tensors (the largest for a workspace)
 inline int norm_bwd_blocks(int64_t rows, int C, int unit_bytes) {
     const NormShape s = norm_shape(C);
-    if (s.nv == 0) return static_cast<int>(rows < 16 ? rows : 16);
+    if (s.nv == 0) {                                                         // strips of rows of the columns' kernel
+        const int64_t most = row_ops_cus() * 4 / ((C + 256 * kUnit - 1) / (256 * kUnit));
+        return static_cast<int>(rows < 8 ? rows : most < 8 ? 8 : rows < most ? rows : most);
+    }
     const int64_t passes = (rows + s.per_block() - 1) / s.per_block();
     if (passes <= 4) return 1;                                               // one workgroup writes the results itself
-    return even_blocks(passes, static_cast<int64_t>(row_ops_cus()) * norm_bwd_per_cu(s, unit_bytes));
+    return even_blocks(passes, static_cast<int64_t>(row_ops_cus()) * norm_bwd_per_cu(s, C, unit_bytes));
 }
 inline int64_t norm_bwd_workspace_floats(int64_t rows, int C) {
     const int blocks = norm_bwd_blocks(rows, C, 16);
@@ -537,10 +539,10 @@ void norm_finish(const NormBwdArgs& a, int blocks, hipStream_t stream);         
 
 namespace {
 
-template <typename T, typename S, bool JOIN, bool RAGGED, typename Run>
+template <typename T, typename S, bool JOIN, int RAGGED, typename Run>
 void norm_fwd_pick(const NormShape& s, Run run) {
     if (s.threads == 0)
-        s.nv == 1 ? run(k_norm_fwd<T, S, JOIN, 1, 0, RAGGED>) : run(k_norm_fwd<T, S, JOIN, 2, 0, RAGGED>);
+        s.nv == 1 ? run(k_norm_fwd<T, S, JOIN, 1, 0, RAGGED ? 1 : 0>) : run(k_norm_fwd<T, S, JOIN, 2, 0, RAGGED>);
     else if (s.threads == 256)
         s.nv == 1 ? run(k_norm_fwd<T, S, JOIN, 1, 256, RAGGED>) : run(k_norm_fwd<T, S, JOIN, 2, 256, RAGGED>);
     else
@@ -557,13 +559,13 @@ void norm_fwd_launch(NormFwdArgs a, hipStream_t stream) {
     if (s.nv == 0)
         run(k_norm_fwd_long<T, S, JOIN>);
     else
-        a.C % kUnit ? norm_fwd_pick<T, S, JOIN, true>(s, run) : norm_fwd_pick<T, S, JOIN, false>(s, run);
+        a.C % kUnit ? norm_fwd_pick<T, S, JOIN, 2>(s, run) : norm_fwd_pick<T, S, JOIN, 0>(s, run);
 }
 
-template <typename T, typename S, bool JOIN, bool RAGGED, typename Run>
+template <typename T, typename S, bool JOIN, int RAGGED, typename Run>
 void norm_bwd_pick(const NormShape& s, Run run) {
     if (s.threads == 0)
-        s.nv == 1 ? run(k_norm_bwd<T, S, JOIN, 1, 0, RAGGED>) : run(k_norm_bwd<T, S, JOIN, 2, 0, RAGGED>);
+        s.nv == 1 ? run(k_norm_bwd<T, S, JOIN, 1, 0, RAGGED ? 1 : 0>) : run(k_norm_bwd<T, S, JOIN, 2, 0, RAGGED>);
     else if (s.threads == 256)
         s.nv == 1 ? run(k_norm_bwd<T, S, JOIN, 1, 256, RAGGED>) : run(k_norm_bwd<T, S, JOIN, 2, 256, RAGGED>);
     else
@@ -587,7 +589,7 @@ void norm_bwd_launch(NormBwdArgs a, hipStream_t stream) {
     }
     const dim3 grid(blocks), block(s.block());
     const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a); };
-    a.C % kUnit ? norm_bwd_pick<T, S, JOIN, true>(s, run) : norm_bwd_pick<T, S, JOIN, false>(s, run);
+    a.C % kUnit ? norm_bwd_pick<T, S, JOIN, 2>(s, run) : norm_bwd_pick<T, S, JOIN, 0>(s, run);
     if (sums && blocks > 1) norm_finish(a, blocks, stream);
 }
 

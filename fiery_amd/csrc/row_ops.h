@@ -78,8 +78,11 @@ __device__ __forceinline__ V pick(bool first, V a, V b) {
 // A unit as it lies in memory: loads are issued well before unpack() makes their values.  `count` (0 .. 8) of its columns belong
 // to the row, the others come out as zeros and nothing past them is touched.  A last unit with fewer than eight is read as the
 // row's last eight columns, so every lane makes the same access, and shifted into place by unpack(); rows narrower than a unit
-// go in pieces.  RAGGED: the width is no multiple of eight; otherwise none of this is compiled in.
-template <bool RAGGED>
+// go in pieces.  RAGGED: the width is no multiple of eight (0: it is, and none of this is compiled in); 1: every wavefront holds last
+// units, all lanes take the shift; 2: few do, and a branch keeps it (and its masks' registers) out of the others;
+// rows are at least a unit wide then.  `live`: whether there is a row
+// at all (apart from `count`, which is then the same for all rows of a lane and its comparisons leave the loop).
+template <int RAGGED>
 __device__ __forceinline__ int unit_count(int C, long long unit) {
     const long long left = C - unit * kUnit;
     return left >= kUnit ? kUnit : RAGGED && left > 0 ? static_cast<int>(left) : 0;
@@ -119,22 +122,22 @@ __device__ __forceinline__ Raw<T> load_pieces(const typename T::store* p, int co
     }
     return r;
 }
-template <typename T, bool RAGGED>
-__device__ __forceinline__ Raw<T> load_raw(const typename T::store* p, int count, int C) {
-    if (RAGGED && C < kUnit) return load_pieces<T>(p, count);
+template <typename T, int RAGGED>
+__device__ __forceinline__ Raw<T> load_raw(const typename T::store* p, bool live, int count, int C) {
+    if (RAGGED == 1 && C < kUnit) return load_pieces<T>(p, live ? count : 0);
     Raw<T> r = {};
-    if (count > 0) {
+    if (live && count > 0) {
         if (RAGGED) p -= kUnit - count;
         __builtin_memcpy(&r.w[0], p, 16);
         if constexpr (sizeof(typename T::store) == 4) __builtin_memcpy(&r.w[4], p + 4, 16);
     }
     return r;
 }
-template <typename T, bool RAGGED>
+template <typename T, int RAGGED>
 __device__ __forceinline__ void unpack(Raw<T> r, int count, int C, float (&v)[kUnit]) {
     constexpr int kWords = sizeof(typename T::store) * kUnit / 4;
-    if (RAGGED && C > kUnit) {
-        const unsigned off = count > 0 ? kUnit - count : 0;
+    const unsigned off = RAGGED && count > 0 ? kUnit - count : 0;
+    if (RAGGED && C > kUnit && (RAGGED == 1 || off)) {
         unsigned words = off;
         if constexpr (kWords == 4) {
 #pragma unroll
@@ -154,12 +157,12 @@ __device__ __forceinline__ void unpack(Raw<T> r, int count, int C, float (&v)[kU
             v[j] = T::value(j & 1 ? r.w[j / 2] >> 16 : r.w[j / 2] & 0xffffu);
     }
 }
-template <typename T, bool RAGGED>
+template <typename T, int RAGGED>
 __device__ __forceinline__ void load_unit(const typename T::store* p, int count, int C, float (&v)[kUnit]) {
-    unpack<T, RAGGED>(load_raw<T, RAGGED>(p, count, C), count, C, v);
+    unpack<T, RAGGED>(load_raw<T, RAGGED>(p, true, count, C), count, C, v);
 }
 // (a store of less than a unit goes in pieces)
-template <typename T, bool RAGGED>
+template <typename T, int RAGGED>
 __device__ __forceinline__ void store_unit(typename T::store* p, int count, const float (&v)[kUnit]) {
     if (RAGGED ? count == kUnit : count > 0) {
         store_n<T, 8>(p, v);
@@ -179,16 +182,17 @@ __device__ __forceinline__ void store_unit(typename T::store* p, int count, cons
 }
 
 // parameters, whose type is known at run time only: read once per lane, outside the loops
+template <int RAGGED>
 __device__ __forceinline__ void load_typed(const void* p, int type, long long c, int count, int C, float otherwise, float (&v)[kUnit]) {
     if (!p) {
 #pragma unroll
         for (int j = 0; j < kUnit; ++j) v[j] = otherwise;
     } else if (type == FIERY_TYPE_F32) {
-        load_unit<F32, true>(static_cast<const float*>(p) + c, count, C, v);
+        load_unit<F32, RAGGED>(static_cast<const float*>(p) + c, count, C, v);
     } else if (type == FIERY_TYPE_BF16) {
-        load_unit<BF16, true>(static_cast<const unsigned short*>(p) + c, count, C, v);
+        load_unit<BF16, RAGGED>(static_cast<const unsigned short*>(p) + c, count, C, v);
     } else {
-        load_unit<F16, true>(static_cast<const unsigned short*>(p) + c, count, C, v);
+        load_unit<F16, RAGGED>(static_cast<const unsigned short*>(p) + c, count, C, v);
     }
 }
 __device__ __forceinline__ void store_typed(void* p, int type, long long i, float v) {
