@@ -1,7 +1,9 @@
-"""Builds libfiery_hip.so (gfx950) in-tree with hipcc.  `python -m fiery_amd.build [--force]`."""
+"""Builds libfiery_hip.so (gfx950) in-tree with hipcc, and _row_autograd.so - the row operators' autograd nodes, host C++ against
+PyTorch's headers - with g++.  `python -m fiery_amd.build [--force]`."""
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
@@ -48,6 +50,19 @@ HIP_ONLY = {name: NO_PACKED_FP32 for name in ('layer_norm.hip', 'dropout.hip', '
 COMMON = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-I' + INCLUDE, '-I' + CSRC, '-x', 'hip']
 
 
+# the row operators' autograd nodes (host code; reaches the library through addresses, so it links against PyTorch only)
+AUTOGRAD_SOURCE = os.path.join(CSRC, 'row_autograd.cpp')
+AUTOGRAD_OUT = os.path.join(HERE, '_row_autograd.so')
+
+
+def _autograd_command():
+    import torch
+    base = os.path.dirname(torch.__file__)
+    return [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden', f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}',
+            '-I' + INCLUDE, f'-I{base}/include', f'-I{base}/include/torch/csrc/api/include', '-I' + sysconfig.get_paths()['include'], AUTOGRAD_SOURCE,
+            '-o', AUTOGRAD_OUT, f'-L{base}/lib', '-ltorch_python', '-ltorch_cpu', '-ltorch', '-lc10']
+
+
 def _stale(target, deps):
     if not os.path.exists(target):
         return True
@@ -78,6 +93,11 @@ def build(force=False, verbose=True):
             if verbose:
                 print(' '.join(cmd), flush=True)
             jobs.append((name, subprocess.Popen(cmd)))       # translation units compile side by side
+    if not variant and (force or _stale(AUTOGRAD_OUT, [AUTOGRAD_SOURCE, os.path.join(INCLUDE, 'fiery_hip.h')])):
+        cmd = _autograd_command()
+        if verbose:
+            print(' '.join(cmd), flush=True)
+        jobs.append(('row_autograd.cpp', subprocess.Popen(cmd)))
     failed = [name for name, proc in jobs if proc.wait() != 0]
     if failed:
         raise RuntimeError('hipcc failed for ' + ', '.join(failed))

@@ -217,6 +217,10 @@ _SIGNATURES = {
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 
+# what csrc/row_autograd.cpp calls, in the order of its `Entries`
+ROW_ENTRIES = ('fiery_last_error', 'fiery_layer_norm_fwd', 'fiery_layer_norm_bwd_workspace_floats', 'fiery_layer_norm_bwd', 'fiery_dropout',
+               'fiery_dropout_add_layer_norm_fwd', 'fiery_dropout_add_layer_norm_bwd')
+
 
 def require_usable_gpu_process(what):
     """The input-pipeline entry points keep the signatures of functions the reference calls inside `Dataset.__getitem__`,
@@ -264,7 +268,7 @@ def warp_flags_of_this_host(h, w):
     return _WARP_FLAGS[key]
 
 
-# `CALL_SINK = []`: every launching entry point of the library is bracketed by HIP events on the current stream and filed as
+# `CALL_SINK = []`: every launching entry point of the library that is called through `Lib` (the row operators are not) is bracketed by HIP events on the current stream and filed as
 # (entry point, start, end) - bench.py's per-kernel table of the pass from images (None: the calls go straight through)
 CALL_SINK = None
 _HOST_ONLY = ('version', 'last_error', 'workspace_', 'occupied_offset', 'packed_floats', '_plan', '_used')
@@ -310,6 +314,8 @@ class Lib:
         for name, (restype, argtypes) in _SIGNATURES.items():
             fn = getattr(self.dll, name)          # AttributeError here = symbol missing from the build
             fn.restype, fn.argtypes = restype, argtypes
+        self._row_entries = (C.c_void_p * len(ROW_ENTRIES))(*[C.cast(getattr(self.dll, name), C.c_void_p).value for name in ROW_ENTRIES])
+        self.row_entries = C.addressof(self._row_entries)
         self.launches_on_gpu = hasattr(self.dll, 'hipLaunchKernel')       # (False: the CPU simulator's build of the sources)
         self.dll = _EntryPoints(self.dll)
         got = self.dll.fiery_abi_version()

@@ -432,10 +432,41 @@ def test_refusals(sim):
         for call in (norm, lambda t: drop(t, 0.5, rng), lambda t: join(t, t)):
             with pytest.raises(ValueError, match='columns'):
                 call(huge.expand(shape))
-    y = norm(x.clone().requires_grad_())
-    with pytest.raises(RuntimeError):                               # gradients of gradients
-        g, = torch.autograd.grad(y.sum(), y.grad_fn.next_functions[0][0].variable, create_graph=True)
-        torch.autograd.grad(g.sum(), y.grad_fn.next_functions[0][0].variable)
+
+
+def test_gradients_of_gradients_are_refused(on):
+    """With create_graph the gradients come out as ever; what would go through them once more is an error, not a wrong number."""
+    rng = row_ops.dropout_rng(0, on.device)
+    for op in (lambda t: row_ops.layer_norm(t, lib=on.lib), lambda t: row_ops.dropout(t, 0.5, rng, lib=on.lib),
+               lambda t: row_ops.dropout_add_layer_norm(t, t, p=0.5, rng=rng, lib=on.lib)[0]):
+        x = make((4, 16), F32, on.device, 100).requires_grad_()
+        want, = torch.autograd.grad((op(x) ** 2).sum(), x)
+        got, = torch.autograd.grad((op(x) ** 2).sum(), x, create_graph=True)
+        assert torch.equal(got, want)
+        with pytest.raises(RuntimeError, match='gradients of gradients'):
+            torch.autograd.grad(got.sum() + x.sum(), x)
+
+
+def test_a_norm_of_a_constant_gradient_is_refused_too(on):
+    """dx depends on x even where the incoming gradient depends on nothing."""
+    x = make((4, 16), F32, on.device, 102).requires_grad_()
+    got, = torch.autograd.grad(row_ops.layer_norm(x, lib=on.lib)[..., 0].sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match='gradients of gradients'):
+        torch.autograd.grad((got ** 2).sum(), x)
+
+
+def test_a_changed_input_is_noticed(on):
+    """Autograd's version check: an input of the backward pass that was written in between is an error."""
+    x = make((4, 16), F32, on.device, 101).requires_grad_()
+    z = x * 1.0
+    y = row_ops.layer_norm(z, lib=on.lib)
+    z += 1.0
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.sum().backward()
+    y, h = row_ops.dropout_add_layer_norm(x, x, lib=on.lib)
+    h += 1.0
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.sum().backward()
 
 
 def test_entry_points_refuse(sim):
@@ -594,25 +625,3 @@ def test_offsets_past_32_bits(hip):
     assert row_ops._rows(far)[1] == 1_200_000_000
     assert torch.equal(row_ops.layer_norm(far), row_ops.layer_norm(far.contiguous()))
     assert torch.equal(row_ops.dropout(far, 0.3, rng, residual=far), row_ops.dropout(far.contiguous(), 0.3, rng, residual=far.contiguous()))
-
-
-def test_calls_go_to_the_tensors_device_and_stream(monkeypatch):
-    """A tensor on another device than the current one: the launch happens with that device current and on its stream."""
-    seen = []
-
-    class Guard:
-        def __init__(self, dev):
-            self.dev = dev
-
-        def __enter__(self):
-            seen.append(('enter', self.dev))
-
-        def __exit__(self, *a):
-            seen.append(('exit', self.dev))
-    monkeypatch.setattr(torch.cuda, 'device', Guard)
-    monkeypatch.setattr(torch._C, '_cuda_getDevice', lambda: 0, raising=False)
-    monkeypatch.setattr(torch._C, '_cuda_getCurrentRawStream', lambda dev: 1000 + dev, raising=False)
-    entry = lambda *args: seen.append(args) or 0
-    for dev in (0, 1):
-        row_ops._launch(None, type('T', (), dict(get_device=lambda self, d=dev: d))(), entry, 'a')
-    assert seen == [('a', 1000), ('enter', 1), ('a', 1001), ('exit', 1)]
