@@ -30,7 +30,7 @@ __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
     for (unsigned long long q = static_cast<unsigned long long>(blockIdx.x) * 256 + threadIdx.x; q < a.total; q += static_cast<unsigned long long>(gridDim.x) * 256) {
         const unsigned row = div_by(static_cast<unsigned>(q), a.units), unit = static_cast<unsigned>(q) - row * a.units.d;
         const long long c = static_cast<long long>(unit) * kUnit;
-        const int count = RAGGED ? unit_count<1>(a.C, unit) : kUnit;
+        const int count = RAGGED ? unit_count<RAGGED>(a.C, unit) : kUnit;
         float v[kUnit];
         load_unit<I, RAGGED>(static_cast<const typename I::store*>(a.x) + row * a.x_ld + c, count, a.C, v);
         if constexpr (RES) {
@@ -49,12 +49,13 @@ __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
 template <typename I, typename O>
 void dropout_launch(const DropoutArgs& a, hipStream_t stream) {
     const dim3 grid(ceil_div(a.total, 256)), block(256);
-    const bool ragged = a.C % kUnit;
     const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a); };
-    if (a.residual)
-        ragged ? run(k_dropout<I, O, true, 1>) : run(k_dropout<I, O, true, 0>);
+    if (a.C < kUnit)
+        a.residual ? run(k_dropout<I, O, true, 3>) : run(k_dropout<I, O, false, 3>);
+    else if (a.C % kUnit)
+        a.residual ? run(k_dropout<I, O, true, 1>) : run(k_dropout<I, O, false, 1>);
     else
-        ragged ? run(k_dropout<I, O, false, 1>) : run(k_dropout<I, O, false, 0>);
+        a.residual ? run(k_dropout<I, O, true, 0>) : run(k_dropout<I, O, false, 0>);
 }
 
 }  // namespace

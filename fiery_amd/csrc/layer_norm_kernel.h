@@ -112,7 +112,7 @@ __device__ __forceinline__ void load_h(const NormFwdArgs& a, const DropKey& key,
 
 template <int RAGGED>
 __device__ __forceinline__ void distances(const float (&v)[kUnit], int count, float mean, float& q) {
-    if (RAGGED == 1 || (RAGGED == 2 && count < kUnit)) {
+    if (RAGGED == 1 || RAGGED == 3 || (RAGGED == 2 && count < kUnit)) {
 #pragma unroll
         for (int j = 0; j < kUnit; ++j) {
             const float d = j < count ? v[j] - mean : 0.f;
@@ -526,7 +526,7 @@ inline int norm_bwd_blocks(int64_t rows, int C, int unit_bytes) {
         return static_cast<int>(rows < 8 ? rows : most < 8 ? 8 : rows < most ? rows : most);
     }
     const int64_t passes = (rows + s.per_block() - 1) / s.per_block();
-    if (passes <= 4) return 1;                                               // one workgroup writes the results itself
+    if (passes <= 8) return 1;                                               // one workgroup writes the results itself
     return even_blocks(passes, static_cast<int64_t>(row_ops_cus()) * norm_bwd_per_cu(s, C, unit_bytes));
 }
 inline int64_t norm_bwd_workspace_floats(int64_t rows, int C) {
@@ -558,6 +558,8 @@ void norm_fwd_launch(NormFwdArgs a, hipStream_t stream) {
     const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a); };
     if (s.nv == 0)
         run(k_norm_fwd_long<T, S, JOIN>);
+    else if (a.C < kUnit)
+        run(k_norm_fwd<T, S, JOIN, 1, 0, 3>);
     else
         a.C % kUnit ? norm_fwd_pick<T, S, JOIN, 2>(s, run) : norm_fwd_pick<T, S, JOIN, 0>(s, run);
 }
@@ -589,7 +591,10 @@ void norm_bwd_launch(NormBwdArgs a, hipStream_t stream) {
     }
     const dim3 grid(blocks), block(s.block());
     const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a); };
-    a.C % kUnit ? norm_bwd_pick<T, S, JOIN, 2>(s, run) : norm_bwd_pick<T, S, JOIN, 0>(s, run);
+    if (a.C < kUnit)
+        run(k_norm_bwd<T, S, JOIN, 1, 0, 3>);
+    else
+        a.C % kUnit ? norm_bwd_pick<T, S, JOIN, 2>(s, run) : norm_bwd_pick<T, S, JOIN, 0>(s, run);
     if (sums && blocks > 1) norm_finish(a, blocks, stream);
 }
 

@@ -202,14 +202,14 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 };
 
 // ---- dropout -----------------------------------------------------------------------------------------------------------------
-Tensor drop(const Tensor& x, const Tensor& residual, at::ScalarType type, const Mask& m, const Tensor& rng, int64_t call, const Tensor& used, const To& to) {
+Tensor drop(const Tensor& x, const Tensor& residual, at::ScalarType type, const Mask& m, const int64_t* rng, int64_t call, int64_t* used, const To& to) {
     const Sizes s = sizes_of(x);
     Tensor y = dense_like(x, type);
     if (s.rows) {
         const auto [xr, ld] = rows_of(x);
         const auto [rr, r_ld] = residual.defined() ? rows_of(residual) : std::pair<Tensor, int64_t>();
         check(to, to.lib->dropout(ptr(xr), ld, type_of(xr), ptr(rr), r_ld, s.rows, static_cast<int>(s.c), static_cast<int>(m.threshold),
-                                  m.threshold ? numbers(rng) : nullptr, call, m.share, static_cast<int>(m.one_column), numbers(used), ptr(y), s.c, type_of(type),
+                                  m.threshold ? rng : nullptr, call, m.share, static_cast<int>(m.one_column), used, ptr(y), s.c, type_of(type),
                                   to.stream));
     }
     return y;
@@ -227,7 +227,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
         const Tensor used = used_numbers(x, m);
         ctx->save_for_backward({used});
         ctx->saved_data[kMeta] = std::vector<int64_t>{static_cast<int64_t>(x.scalar_type()), threshold, share, one_column, entries, stream, residual.defined()};
-        return drop(x, residual, residual.defined() ? residual.scalar_type() : x.scalar_type(), m, or_none(rng), call, used, to_of(entries, stream));
+        return drop(x, residual, residual.defined() ? residual.scalar_type() : x.scalar_type(), m, numbers(or_none(rng)), call, numbers(used), to_of(entries, stream));
     }
     static variable_list backward(AutogradContext* ctx, variable_list incoming) {
         const variable_list saved = ctx->get_saved_variables();
@@ -237,7 +237,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
             const OnDevice on(incoming[0]);
             Tensor dx, dr;
             if (ctx->needs_input_grad(0))
-                dx = drop(incoming[0], Tensor(), static_cast<at::ScalarType>(meta[0]), {meta[1], meta[2], meta[3]}, used, 0, Tensor(), to_of(meta[4], meta[5]));
+                dx = drop(incoming[0], Tensor(), static_cast<at::ScalarType>(meta[0]), {meta[1], meta[2], meta[3]}, numbers(used), 0, nullptr, to_of(meta[4], meta[5]));
             if (meta[6] && ctx->needs_input_grad(1)) dr = incoming[0];
             return {dx, dr, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
         });
@@ -245,8 +245,11 @@ struct Dropout : torch::autograd::Function<Dropout> {
 };
 
 // ---- residual + dropout + layer norm --------------------------------------------------------------------------------------------
+// stats: mean and rstd of the rows, then the two numbers that the masks were drawn with; undefined where no backward pass follows
+int64_t* used_behind(const Tensor& stats, int64_t rows) { return reinterpret_cast<int64_t*>(floats(stats, 2 * rows)); }
+
 variable_list join_forward(const Tensor& x, const Tensor& residual, const Tensor& weight, const Tensor& bias, const Tensor& rng, const Mask& m, int64_t call,
-                           double eps, const To& to, const Tensor& stats, const Tensor& used) {
+                           double eps, const To& to, const Tensor& stats) {
     const Sizes s = sizes_of(x);
     Tensor y = dense_like(x, x.scalar_type()), h = dense_like(x, residual.scalar_type());
     if (s.rows) {
@@ -255,7 +258,7 @@ variable_list join_forward(const Tensor& x, const Tensor& residual, const Tensor
         const Tensor& params = weight.defined() ? weight : bias;
         check(to, to.lib->join_fwd(ptr(xr), ld, type_of(xr), ptr(rr), r_ld, type_of(rr), s.rows, static_cast<int>(s.c), ptr(weight), ptr(bias),
                                    params.defined() ? type_of(params) : 0, static_cast<float>(eps), static_cast<int>(m.threshold),
-                                   m.threshold ? numbers(rng) : nullptr, call, m.share, static_cast<int>(m.one_column), numbers(used), ptr(y), s.c, ptr(h), s.c,
+                                   m.threshold ? numbers(rng) : nullptr, call, m.share, static_cast<int>(m.one_column), used_behind(stats, s.rows), ptr(y), s.c, ptr(h), s.c,
                                    floats(stats), floats(stats, s.rows), to.stream));
     }
     return {y, h};
@@ -266,29 +269,30 @@ struct DropoutAddLayerNorm : torch::autograd::Function<DropoutAddLayerNorm> {
                                  int64_t threshold, int64_t share, int64_t one_column, int64_t call, double eps, int64_t entries, int64_t stream) {
         const Tensor weight = or_none(weight_), bias = or_none(bias_);
         const Mask m{threshold, share, one_column};
-        const Tensor used = used_numbers(x, m), stats = at::empty({2 * sizes_of(x).rows}, x.options().dtype(at::kFloat).requires_grad(false));
-        variable_list out = join_forward(x, residual, weight, bias, or_none(rng), m, call, eps, to_of(entries, stream), stats, used);
+        const Tensor stats = at::empty({2 * sizes_of(x).rows + 4}, x.options().dtype(at::kFloat).requires_grad(false));
+        variable_list out = join_forward(x, residual, weight, bias, or_none(rng), m, call, eps, to_of(entries, stream), stats);
         ctx->set_materialize_grads(false);
-        ctx->save_for_backward({out[1], weight, stats, used});
+        ctx->save_for_backward({out[1], weight, stats});
         ctx->saved_data[kMeta] = std::vector<int64_t>{static_cast<int64_t>(x.scalar_type()), type_or_none(bias), threshold, share, one_column, entries, stream};
         return out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list incoming) {
         const variable_list saved = ctx->get_saved_variables();
         return once(incoming, saved, [&]() -> variable_list {
-            const Tensor &h = saved[0], &weight = saved[1], &stats = saved[2], &used = saved[3];
+            const Tensor &h = saved[0], &weight = saved[1], &stats = saved[2];
             const auto meta = ctx->saved_data[kMeta].toIntVector();
             const auto x_type = static_cast<at::ScalarType>(meta[0]);
             const Mask m{meta[2], meta[3], meta[4]};
             const To to = to_of(meta[5], meta[6]);
             const OnDevice on(h);
             Sizes s = sizes_of(h);
+            int64_t* const used = used_behind(stats, s.rows);
             const Tensor &dy = incoming[0], &dh = incoming[1];
             const bool want_x = ctx->needs_input_grad(0), want_r = ctx->needs_input_grad(1);
             Tensor dx, dr;
             if (!dy.defined()) {                                        // only h went on: there is no norm to differentiate
                 s.rows = 0;
-                if (want_x && dh.defined()) dx = drop(dh, Tensor(), x_type, m, used, 0, Tensor(), to);
+                if (want_x && dh.defined()) dx = drop(dh, Tensor(), x_type, m, used, 0, nullptr, to);
                 if (want_r) dr = dh;
             } else {
                 if (want_x) dx = dense_like(h, x_type);
@@ -300,7 +304,7 @@ struct DropoutAddLayerNorm : torch::autograd::Function<DropoutAddLayerNorm> {
                 const auto [hg, dh_ld] = dh.defined() ? rows_of(dh) : std::pair<Tensor, int64_t>();
                 check(to, to.lib->join_bwd(ptr(gr), dy_ld, ptr(hg), dh_ld, ptr(h), s.c, type_of(x_type), type_of(h), s.rows, static_cast<int>(s.c), ptr(weight),
                                            weight.defined() ? type_of(weight) : p.type, floats(stats), floats(stats, s.rows), static_cast<int>(m.threshold),
-                                           numbers(used), m.share, static_cast<int>(m.one_column), ptr(dx), s.c, ptr(dr), s.c, ptr(p.dw), ptr(p.db),
+                                           used, m.share, static_cast<int>(m.one_column), ptr(dx), s.c, ptr(dr), s.c, ptr(p.dw), ptr(p.db),
                                            floats(p.workspace), p.floats, to.stream));
             } else {
                 p.zero();
@@ -325,22 +329,22 @@ Tensor layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, doubl
 Tensor dropout(const Tensor& x, const Maybe& residual, const Maybe& rng, const std::tuple<int64_t, int64_t, int64_t>& mask, int64_t call, int64_t entries,
                int64_t stream) {
     const OnDevice on(x);
-    const Tensor r = residual.value_or(Tensor()), numbers = rng.value_or(Tensor());
+    const Tensor r = or_none(residual);
     const auto [threshold, share, one_column] = mask;
-    if (at::GradMode::is_enabled() && (wants(x) || wants(r))) return Dropout::apply(x, maybe(r), maybe(numbers), threshold, share, one_column, call, entries, stream);
-    return drop(x, r, r.defined() ? r.scalar_type() : x.scalar_type(), {threshold, share, one_column}, numbers, call, Tensor(), to_of(entries, stream));
+    if (at::GradMode::is_enabled() && (wants(x) || wants(r))) return Dropout::apply(x, residual, rng, threshold, share, one_column, call, entries, stream);
+    return drop(x, r, r.defined() ? r.scalar_type() : x.scalar_type(), {threshold, share, one_column}, numbers(or_none(rng)), call, nullptr, to_of(entries, stream));
 }
 
 std::pair<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const Tensor& residual, const Maybe& weight, const Maybe& bias, const Maybe& rng,
                                                  const std::tuple<int64_t, int64_t, int64_t>& mask, int64_t call, double eps, int64_t entries, int64_t stream) {
     const OnDevice on(x);
-    const Tensor w = dense(weight), b = dense(bias), numbers = rng.value_or(Tensor());
+    const Tensor w = dense(weight), b = dense(bias);
     const auto [threshold, share, one_column] = mask;
     variable_list out;
     if (at::GradMode::is_enabled() && (wants(x) || wants(residual) || wants(w) || wants(b)))
-        out = DropoutAddLayerNorm::apply(x, residual, maybe(w), maybe(b), maybe(numbers), threshold, share, one_column, call, eps, entries, stream);
+        out = DropoutAddLayerNorm::apply(x, residual, maybe(w), maybe(b), rng, threshold, share, one_column, call, eps, entries, stream);
     else
-        out = join_forward(x, residual, w, b, numbers, {threshold, share, one_column}, call, eps, to_of(entries, stream), Tensor(), Tensor());
+        out = join_forward(x, residual, w, b, or_none(rng), {threshold, share, one_column}, call, eps, to_of(entries, stream), Tensor());
     return {out[0], out[1]};
 }
 

@@ -79,8 +79,8 @@ __device__ __forceinline__ V pick(bool first, V a, V b) {
 // to the row, the others come out as zeros and nothing past them is touched.  A last unit with fewer than eight is read as the
 // row's last eight columns, so every lane makes the same access, and shifted into place by unpack(); rows narrower than a unit
 // go in pieces.  RAGGED: the width is no multiple of eight (0: it is, and none of this is compiled in); 1: every wavefront holds last
-// units, all lanes take the shift; 2: few do, and a branch keeps it (and its masks' registers) out of the others;
-// rows are at least a unit wide then.  `live`: whether there is a row
+// units, all lanes take the shift; 2: few do, and a branch keeps it (and its masks' registers) out of the others; 3:
+// rows narrower than a unit.  `live`: whether there is a row
 // at all (apart from `count`, which is then the same for all rows of a lane and its comparisons leave the loop).
 template <int RAGGED>
 __device__ __forceinline__ int unit_count(int C, long long unit) {
@@ -124,7 +124,7 @@ __device__ __forceinline__ Raw<T> load_pieces(const typename T::store* p, int co
 }
 template <typename T, int RAGGED>
 __device__ __forceinline__ Raw<T> load_raw(const typename T::store* p, bool live, int count, int C) {
-    if (RAGGED == 1 && C < kUnit) return load_pieces<T>(p, live ? count : 0);
+    if (RAGGED == 3) return load_pieces<T>(p, live ? count : 0);
     Raw<T> r = {};
     if (live && count > 0) {
         if (RAGGED) p -= kUnit - count;
@@ -136,8 +136,8 @@ __device__ __forceinline__ Raw<T> load_raw(const typename T::store* p, bool live
 template <typename T, int RAGGED>
 __device__ __forceinline__ void unpack(Raw<T> r, int count, int C, float (&v)[kUnit]) {
     constexpr int kWords = sizeof(typename T::store) * kUnit / 4;
-    const unsigned off = RAGGED && count > 0 ? kUnit - count : 0;
-    if (RAGGED && C > kUnit && (RAGGED == 1 || off)) {
+    const unsigned off = (RAGGED == 1 || RAGGED == 2) && count > 0 ? kUnit - count : 0;
+    if (RAGGED == 1 || (RAGGED == 2 && off)) {
         unsigned words = off;
         if constexpr (kWords == 4) {
 #pragma unroll
