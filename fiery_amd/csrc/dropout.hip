@@ -6,6 +6,9 @@
 // Memory-bound: x [and the residual] read once, y written once.  The generator costs 20 wide integer multiplications per unit
 // of eight columns, beside 16 or 32 bytes in and out.  Units are dealt to lanes flat over (row, unit), so narrow rows fill
 // their wavefronts; the split of the flat index is one multiplication.
+//
+// Measured (one MI355X; a large copy reaches 5.35 TB/s): 16,384 x 4096 bf16 48 us = 5.6 TB/s; 480,000 x 64 fp32 per channel with a
+// residual 69 us = 5.4 TB/s, its backward pass 43 us = 5.7 TB/s; 90,720 x 56 fp32 per image 12 us = 5.2 TB/s.
 #include "row_ops.h"
 
 namespace fiery {

@@ -14,7 +14,8 @@ The dropout mask is a function of (seed, call, row, column) - Philox4x32-10 (Sal
 p is drawn as round(65536 p) / 65536 and what is kept is scaled by the inverse of exactly that.  `rng` is a device tensor
 int64 [seed, call] (`dropout_rng`); `call=` is added to its second number.  Give every dropout of a step its own number and
 advance the tensor between steps (`rng[1] += calls_per_step`, also inside a captured graph: replays then draw new masks).  The
-forward pass keeps the two numbers it used, so the backward pass draws the same mask whatever happens to `rng` in between.
+forward pass keeps the two numbers it used, so the backward pass draws the same mask whatever happens to `rng` in between (activation
+checkpointing runs the forward pass again: advance `rng` after the backward pass there).
 
 Only `p = 0` works without an `rng`.  Gradients of gradients are not provided.  The autograd nodes are csrc/row_autograd.cpp; here are
 the arguments and their checks."""
