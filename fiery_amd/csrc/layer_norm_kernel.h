@@ -18,8 +18,8 @@
 //
 // Measured (one MI355X; a large copy reaches 5.35 TB/s): 480,000 x 64 fp32 forward 46 us = 5.4 TB/s, backward 69 + 5 us = 5.0 TB/s,
 // joined 94 and 120 + 5 us = 5.2 and 4.9 TB/s; 8192 x 4096 bf16 28 and 39 + 4 us = 4.7 TB/s, joined 53 and 63 + 5 us = 5.1 and 5.0 TB/s;
-// 90,720 x 128 fp16 forward 11 us = 4.1 TB/s.  Counter traffic is the operands' and the partial rows'.  240,000 x 35 bf16: 15 and 20 + 5 us
-// = 2.3 and 2.0 TB/s, bound by instructions (five of a group's eight lanes hold columns).
+// 90,720 x 128 fp16 forward 11 us = 4.1 TB/s.  Counter traffic is the operands' and the partial rows'.  240,000 x 35 bf16: 14 and 18 + 5 us
+// = 2.4 and 2.1 TB/s, bound by instructions (five of a group's eight lanes hold columns).
 #pragma once
 #include "row_ops.h"
 
