@@ -512,12 +512,13 @@ inline int even_blocks(int64_t passes, int64_t most) {
 // Workgroups per CU.  More of them than it takes to keep memory busy cost: the streams' pages are spread wider (forward, 64 fp32
 // columns: 44 us with 2, 48 with 8 for 480,000 rows), and every workgroup of the backward pass leaves a partial row (4096 bf16
 // columns, 8192 rows: 44 us with 1, 55 with 4).  Forward: 512 lanes with 32 bytes or 1024 with 16 (4096 bf16 columns: 36 us with
-// 1 workgroup, 24 with 4); ragged widths, which are bound by their arithmetic, twice that.  Backward, whose next row is on its
+// 1 workgroup, 24 with 4; 101 fp32, joined: 57 with 2, 60 with 4); half as many again for ragged 16-bit rows of one unit a lane, which
+// are bound by their arithmetic (501 bf16, joined: 58 with 6, 64 with 4, 63 with 8).  Backward, whose next row is on its
 // way already: 16 KB of each tensor in flight where wavefronts hold the rows (bf16, 64 columns: 73 us with 1, 39 with 4, 44 with 8), 8 KB
 // where workgroups do.
 inline int norm_fwd_per_cu(const NormShape& s, int C, int unit_bytes) {
-    const int n = (C % kUnit ? 2 : 1) * 16384 / unit_bytes / s.block();
-    return n < 2 ? 2 : n;
+    const int n = 16384 / unit_bytes / s.block();
+    return n < 2 ? 2 : C % kUnit && s.nv == 1 && unit_bytes == 16 ? n + n / 2 : n;
 }
 inline int norm_bwd_per_cu(const NormShape& s, int C, int unit_bytes) {
     const int n = (C % kUnit && s.threads ? 2 : 1) * (s.threads ? 8192 : 16384) / (s.block() * s.nv * unit_bytes);
