@@ -625,3 +625,56 @@ def test_offsets_past_32_bits(hip):
     assert row_ops._rows(far)[1] == 1_200_000_000
     assert torch.equal(row_ops.layer_norm(far), row_ops.layer_norm(far.contiguous()))
     assert torch.equal(row_ops.dropout(far, 0.3, rng, residual=far), row_ops.dropout(far.contiguous(), 0.3, rng, residual=far.contiguous()))
+
+
+def test_errors_of_the_library_and_of_the_build_are_told(sim, monkeypatch):
+    """A refusal of an entry point comes out with its text, in the forward and in the backward pass; a missing build says what to do."""
+    import ctypes
+    table = (ctypes.c_void_p * len(native.ROW_ENTRIES))(*sim._row_entries)
+    answer = {'rc': 0}
+    signature = ctypes.CFUNCTYPE(*[native._SIGNATURES['fiery_dropout'][0], *native._SIGNATURES['fiery_dropout'][1]])
+    refuse = signature(lambda *args: answer['rc'])
+    table[native.ROW_ENTRIES.index('fiery_dropout')] = ctypes.cast(refuse, ctypes.c_void_p).value
+    lib = type('Lib', (), dict(launches_on_gpu=False, row_entries=ctypes.addressof(table)))()
+    sim.dll.fiery_dropout(None, 0, 0, None, 0, 1, 1, 0, None, 0, 1, 0, None, None, 0, 0, None)           # leaves 'dropout: null pointer'
+    x = torch.ones(2, 8, requires_grad=True)
+    rng = row_ops.dropout_rng(0, 'cpu')
+    y = row_ops.dropout(x, 0.5, rng, lib=lib)
+    answer['rc'] = -22
+    with pytest.raises(RuntimeError, match='error -22: dropout: null pointer'):
+        row_ops.dropout(x, 0.5, rng, lib=lib)
+    with pytest.raises(RuntimeError, match='error -22'):
+        y.sum().backward()
+    monkeypatch.setattr(row_ops, '_nodes', None)
+    monkeypatch.setitem(sys.modules, 'fiery_amd._row_autograd', None)
+    monkeypatch.delattr('fiery_amd._row_autograd', raising=False)
+    with pytest.raises(native.NativeError, match='build it first'):
+        row_ops.layer_norm(x, lib=sim)
+
+
+def test_activation_checkpointing_draws_the_same_masks(on):
+    """The forward pass run again inside the backward pass: the same numbers, as long as rng stays."""
+    from torch.utils.checkpoint import checkpoint
+    x = make((4, 24), F32, on.device, 110).requires_grad_()
+    rng = row_ops.dropout_rng(12, on.device)
+
+    def block(t):
+        y, h = row_ops.dropout_add_layer_norm(torch.tanh(t), t, p=0.4, rng=rng, lib=on.lib)
+        return row_ops.dropout(y, 0.3, rng, call=1, residual=h, lib=on.lib)
+    want, = torch.autograd.grad(block(x).square().sum(), x)
+    got, = torch.autograd.grad(checkpoint(block, x, use_reentrant=False).square().sum(), x)
+    assert torch.equal(got, want)
+
+
+def test_widest_and_narrowest_parameters(on):
+    """Parameters that are views: strided, and one value expanded over the columns (its gradient is the sum)."""
+    x, dy = make((9, 40), F32, on.device, 111), make((9, 40), F32, on.device, 112)
+    wide = make((80,), F32, on.device, 113, 0.2, 1.0).requires_grad_()
+    one = make((1,), F32, on.device, 114).requires_grad_()
+    y = row_ops.layer_norm(x, wide[::2], one.expand(40), lib=on.lib)
+    check_norm_forward(y, x.double().cpu(), wide.detach()[::2], one.detach().expand(40), 1e-5)
+    dw, db = torch.autograd.grad(y, (wide, one), dy)
+    _, gw, gb = norm_grads(dy.double().cpu(), x.double().cpu(), wide.detach()[::2], 1e-5)
+    check_stored(dw[::2], gw)
+    assert not dw[1::2].any()
+    check_stored(db, (gb[0].sum(0, keepdim=True), gb[1].sum(0, keepdim=True) + 40 * U * gb[0].abs().sum(0, keepdim=True)))

@@ -134,3 +134,45 @@ def test_model_keeps_its_numbers_and_its_checkpoint(sim):
     third = tg.TrainGraph(None, sim)
     third.m = types.SimpleNamespace()
     assert torch.equal(third.dropout_add(x, torch.zeros_like(x), 0.5, 'channel'), y)
+
+
+@pytest.mark.gpu
+def test_a_models_training_pass_with_dropout(hip):
+    """p > 0 in every Bottleneck of the tiny model: one number per block and pass, finite gradients everywhere, the same outputs from
+    the same numbers (to the rounding of the pooling's atomics: 2e-4 of the largest value, as the suite's other training passes), others
+    from the next."""
+    from fiery_amd.model import Fiery
+    from tests.golden.make_golden import training_loss, training_model_case
+    from tests.helpers import forward_case, randomise_weights
+    cfg, B, n_cam = training_model_case()
+    torch.manual_seed(0)
+    model = Fiery(cfg)
+    randomise_weights(model)
+    keys = list(model.state_dict())
+    model = model.cuda().train()
+    blocks = [m for m in model.modules() if isinstance(m, ResidualBottleneck)]
+    for b in blocks:
+        b.layers.dropout.p = 0.1
+    lifted, K, E, ego, labels, noise = forward_case(cfg, model.receptive_field, model.n_future, model.depth_channels, model.bev_size, B, n_cam,
+                                                    with_labels=True, with_noise=True)
+    args = [t.cuda() for t in (lifted, K, E, ego, labels, noise)]
+
+    def run(call):
+        model.dropout_rng = row_ops.dropout_rng(77)
+        model.dropout_rng[1] = call
+        with torch.no_grad():
+            for m in model.modules():                                # the running averages do not enter a pass in train() mode
+                if isinstance(m, torch.nn.modules.batchnorm._BatchNorm):
+                    m.reset_running_stats()
+        return model.bev_forward(*args)
+    out = run(0)
+    assert model.dropout_rng.tolist() == [77, len(blocks)] and len(blocks) > 8
+    training_loss(out).backward()
+    grads = [p.grad for n, p in model.named_parameters() if not n.startswith('encoder.') and p.grad is not None]
+    assert len(grads) > 100 and all(torch.isfinite(g).all() for g in grads)
+    same, other = run(0), run(len(blocks))
+    a, b, c = (o['instance_offset'].detach() for o in (out, same, other))
+    scale = a.abs().max()
+    assert (a - b).abs().max() <= 2e-4 * max(1.0, scale)
+    assert (a - c).abs().max() > 1e-2 * scale
+    assert list(model.state_dict()) == keys
