@@ -15,6 +15,9 @@
 // With a 16-bit stream y comes from the h before its rounding, while the statistics that are kept are those of the h that is
 // stored, which is what the backward pass reads: its xhat then sums to zero and has its variance, and the gradient is the norm's
 // at that h.  (With the other statistics a row of small variance beside a large mean had an xhat off by |mean| rstd / 256.)
+// That gradient carries h's rounding: dgamma's error grows with |mean| rstd.  SUM (16-bit streams, the caller's choice): the backward
+// pass makes h again from x and residual, unrounded, under the statistics of that h; one tensor more to read (480,000 x 64 bf16: 82 us
+// against 65; 8192 x 4096 bf16: 90 - 95 against 73 - 80, both with the sum of the partial rows).
 //
 // Measured (one MI355X; a large copy reaches 5.35 TB/s): 480,000 x 64 fp32 forward 46 us = 5.4 TB/s, backward 69 + 5 us = 5.0 TB/s,
 // joined 94 and 120 + 5 us = 5.2 and 4.9 TB/s; 8192 x 4096 bf16 28 and 39 + 4 us = 4.7 TB/s, joined 53 and 63 + 5 us = 5.1 and 5.0 TB/s;
@@ -37,13 +40,15 @@ struct NormFwdArgs {
     long long x_ld, res_ld, y_ld, h_ld;
     int rows, C, lane_bits, param_type;
     float eps, inv_c;
+    int of_sum;                          // mean, rstd: of the h before its rounding (a backward pass with x and residual follows)
     DropArgs drop;
 };
 
 struct NormBwdArgs {
     const void* dy;
     const void* dh;                      // JOIN: gradient of h itself, may be null
-    const void* h;                       // the rows that were normalised (alone: x)
+    const void* h;                       // the rows that were normalised (alone: x; SUM: the residual)
+    const void* x;                       // SUM only
     const void* gamma;
     const float* mean;
     const float* rstd;
@@ -52,7 +57,7 @@ struct NormBwdArgs {
     float* partial;                      // [workgroups][2][round_up(C, 8)]: dgamma, dbeta of a workgroup's rows; null: not wanted
     void* dgamma;                        // written here by a single workgroup
     void* dbeta;
-    long long dy_ld, dh_ld, h_ld, dx_ld, dres_ld;
+    long long dy_ld, dh_ld, h_ld, x_ld, dx_ld, dres_ld;
     int rows, C, lane_bits, param_type;
     float inv_c;
     DropArgs drop;
@@ -190,8 +195,9 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_fwd(NormFwdArg
         row_sums<THREADS>(q, lanes, slots, turn);
         const float rstd = rstd_of(q[0] * a.inv_c + a.eps);
         if (a.mean && live && sub == 0) {
-            a.mean[row] = two ? mean_of(s[two ? 1 : 0], a.C, a.inv_c) : mean;
-            a.rstd[row] = two ? rstd_of(q[two ? 1 : 0] * a.inv_c + a.eps) : rstd;
+            const bool stored = two && !a.of_sum;
+            a.mean[row] = stored ? mean_of(s[two ? 1 : 0], a.C, a.inv_c) : mean;
+            a.rstd[row] = stored ? rstd_of(q[two ? 1 : 0] * a.inv_c + a.eps) : rstd;
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -239,8 +245,9 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_long(NormFwdArgs a) {
         row_sums<1024>(q, 64, slots, turn);
         const float rstd = rstd_of(q[0] * a.inv_c + a.eps);
         if (a.mean && threadIdx.x == 0) {
-            a.mean[row] = two ? mean_of(s[two ? 1 : 0], a.C, a.inv_c) : mean;
-            a.rstd[row] = two ? rstd_of(q[two ? 1 : 0] * a.inv_c + a.eps) : rstd;
+            const bool stored = two && !a.of_sum;
+            a.mean[row] = stored ? mean_of(s[two ? 1 : 0], a.C, a.inv_c) : mean;
+            a.rstd[row] = stored ? rstd_of(q[two ? 1 : 0] * a.inv_c + a.eps) : rstd;
         }
         for (int u = threadIdx.x; u < units; u += blockDim.x) {
             const int count = unit_count<2>(a.C, u);
@@ -255,10 +262,25 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_long(NormFwdArgs a) {
     }
 }
 
+// SUM: the unit of h from the residual's (in v) and x's; -> which of its columns are kept
+template <typename T, int RAGGED>
+__device__ __forceinline__ unsigned sum_again(const NormBwdArgs& a, const DropKey& key, long long row, int unit, int count, const Raw<T>& x, float (&v)[kUnit]) {
+    float d[kUnit];
+    unpack<T, RAGGED>(x, count, a.C, d);
+    unsigned bits = 0;
+    if (a.drop.threshold) {
+        bits = drop_bits(a.drop, key, static_cast<unsigned>(row), static_cast<unsigned>(unit));
+        drop_by(a.drop, bits, d);
+    }
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j) v[j] = d[j] + v[j];
+    return bits;
+}
+
 // One unit of the backward pass's results from its dy (gg = dy gamma), xhat and the row's sums.
-template <typename T, typename S, bool JOIN, int RAGGED>
+template <typename T, typename S, bool JOIN, int RAGGED, bool SUM>
 __device__ __forceinline__ void store_grads(const NormBwdArgs& a, const DropKey& key, long long row, int unit, int count, const float (&gg)[kUnit],
-                                            const float (&xhat)[kUnit], const Raw<S>& dh, float rstd, float m1, float m2) {
+                                            const float (&xhat)[kUnit], const Raw<S>& dh, unsigned bits, float rstd, float m1, float m2) {
     const long long c = static_cast<long long>(unit) * kUnit;
     float out[kUnit];
 #pragma unroll
@@ -272,14 +294,17 @@ __device__ __forceinline__ void store_grads(const NormBwdArgs& a, const DropKey&
         }
         if (a.dres) store_unit<S, RAGGED>(static_cast<typename S::store*>(a.dres) + row * a.dres_ld + c, count, out);
         if (!a.dx) return;
-        drop_unit(a.drop, key, static_cast<unsigned>(row), static_cast<unsigned>(unit), out);
+        if constexpr (!SUM)
+            drop_unit(a.drop, key, static_cast<unsigned>(row), static_cast<unsigned>(unit), out);
+        else if (a.drop.threshold)
+            drop_by(a.drop, bits, out);
     } else {
         if (!a.dx) return;
     }
     store_unit<T, RAGGED>(static_cast<typename T::store*>(a.dx) + row * a.dx_ld + c, count, out);
 }
 
-template <typename T, typename S, bool JOIN, int NV, int THREADS, int RAGGED>
+template <typename T, typename S, bool JOIN, int NV, int THREADS, int RAGGED, bool SUM>
 __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_bwd(NormBwdArgs a) {
     typedef typename std::conditional<JOIN, S, T>::type H;
     __shared__ float slots[2][2][16];
@@ -305,6 +330,7 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_bwd(NormBwdArg
     Raw<H> h_next[NV];
     Raw<T> g_next[NV];
     Raw<S> d_next[NV] = {};
+    Raw<T> x_next[SUM ? NV : 1] = {};
     float mean_next = 0.f, rstd_next = 0.f;
     const auto fetch = [&](long long first) {
         const long long row = first + mine;
@@ -315,6 +341,7 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_bwd(NormBwdArg
             const int unit = i * lanes + sub;
             h_next[i] = load_raw<H, RAGGED>(static_cast<const typename H::store*>(a.h) + at * a.h_ld + static_cast<long long>(unit) * kUnit, live, count[i], a.C);
             g_next[i] = load_raw<T, RAGGED>(static_cast<const typename T::store*>(a.dy) + at * a.dy_ld + static_cast<long long>(unit) * kUnit, live, count[i], a.C);
+            if constexpr (SUM) x_next[i] = load_raw<T, RAGGED>(static_cast<const typename T::store*>(a.x) + at * a.x_ld + static_cast<long long>(unit) * kUnit, live, count[i], a.C);
             if (JOIN && a.dh) d_next[i] = load_raw<S, RAGGED>(static_cast<const typename S::store*>(a.dh) + at * a.dh_ld + static_cast<long long>(unit) * kUnit, live, count[i], a.C);
         }
         mean_next = live ? a.mean[row] : 0.f;                                      // (a row that is none has xhat 0, whatever row 0 holds)
@@ -329,10 +356,12 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_bwd(NormBwdArg
         const float mean = mean_next, rstd = rstd_next;
         float gg[NV][kUnit], xhat[NV][kUnit], s[2] = {0.f, 0.f};
         Raw<S> dh[NV];
+        unsigned bits[NV] = {};
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             dh[i] = d_next[i];
             unpack<H, RAGGED>(h_next[i], count[i], a.C, xhat[i]);
+            if constexpr (SUM) bits[i] = sum_again<T, RAGGED>(a, key, at, i * lanes + sub, count[i], x_next[i], xhat[i]);
             unpack<T, RAGGED>(g_next[i], count[i], a.C, gg[i]);
         }
         if (first + step < a.rows) fetch(first + step);
@@ -351,7 +380,7 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_bwd(NormBwdArg
         const float m1 = s[0] * a.inv_c, m2 = s[1] * a.inv_c;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (live && count[i]) store_grads<T, S, JOIN, RAGGED>(a, key, at, i * lanes + sub, count[i], gg[i], xhat[i], dh[i], rstd, m1, m2);
+            if (live && count[i]) store_grads<T, S, JOIN, RAGGED, SUM>(a, key, at, i * lanes + sub, count[i], gg[i], xhat[i], dh[i], bits[i], rstd, m1, m2);
     }
     if (!a.partial && !a.dgamma && !a.dbeta) return;
     const int width = (a.C + kUnit - 1) / kUnit * kUnit;
@@ -407,7 +436,7 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_bwd(NormBwdArg
 }
 
 // Rows past the registers: the row's sums in one walk, its results in a second; dgamma and dbeta in k_norm_bwd_cols_long.
-template <typename T, typename S, bool JOIN>
+template <typename T, typename S, bool JOIN, bool SUM>
 __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormBwdArgs a) {
     typedef typename std::conditional<JOIN, S, T>::type H;
     __shared__ float slots[2][2][16];
@@ -425,6 +454,11 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormBwdArgs a) {
                 const int count = unit_count<2>(a.C, u);
                 const long long c = static_cast<long long>(u) * kUnit;
                 load_unit<H, 2>(static_cast<const typename H::store*>(a.h) + row * a.h_ld + c, count, a.C, xhat);
+                unsigned bits = 0;
+                if constexpr (SUM) {
+                    const Raw<T> x = load_raw<T, 2>(static_cast<const typename T::store*>(a.x) + row * a.x_ld + c, true, count, a.C);
+                    bits = sum_again<T, 2>(a, key, row, u, count, x, xhat);
+                }
                 load_unit<T, 2>(static_cast<const typename T::store*>(a.dy) + row * a.dy_ld + c, count, a.C, gg);
                 float ga[kUnit];
                 load_typed<2>(a.gamma, a.param_type, c, count, a.C, 1.f, ga);
@@ -442,7 +476,7 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormBwdArgs a) {
                 } else {
                     Raw<S> dh = {};
                     if (JOIN && a.dh) dh = load_raw<S, 2>(static_cast<const typename S::store*>(a.dh) + row * a.dh_ld + c, true, count, a.C);
-                    store_grads<T, S, JOIN, 2>(a, key, row, u, count, gg, xhat, dh, rstd, m1, m2);
+                    store_grads<T, S, JOIN, 2, SUM>(a, key, row, u, count, gg, xhat, dh, bits, rstd, m1, m2);
                 }
             }
             if (walk == 0) row_sums<1024>(s, 64, slots, turn);
@@ -451,15 +485,22 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormBwdArgs a) {
 }
 
 // dgamma, dbeta of one unit of columns over the strip blockIdx.y of the rows, one partial row per strip
-template <typename T, typename H>
+template <typename T, typename H, bool SUM>
 __global__ __launch_bounds__(256) void k_norm_bwd_cols_long(NormBwdArgs a) {
     const int unit = blockIdx.x * 256 + threadIdx.x, count = unit_count<2>(a.C, unit);
     if (count == 0) return;
     const int width = (a.C + kUnit - 1) / kUnit * kUnit;
     const long long c = static_cast<long long>(unit) * kUnit;
     float dg[kUnit] = {}, db[kUnit] = {}, h[kUnit], g[kUnit];
+    DropKey key = {0, 0, 0, 0};
+    if constexpr (SUM)
+        if (a.drop.threshold) key = drop_key(a.drop);
     for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
         load_unit<H, 2>(static_cast<const typename H::store*>(a.h) + row * a.h_ld + c, count, a.C, h);
+        if constexpr (SUM) {
+            const Raw<T> x = load_raw<T, 2>(static_cast<const typename T::store*>(a.x) + row * a.x_ld + c, true, count, a.C);
+            sum_again<T, 2>(a, key, row, unit, count, x, h);
+        }
         load_unit<T, 2>(static_cast<const typename T::store*>(a.dy) + row * a.dy_ld + c, count, a.C, g);
         const float mean = a.mean[row], rstd = a.rstd[row];
 #pragma unroll
@@ -570,16 +611,16 @@ void norm_fwd_launch(NormFwdArgs a, hipStream_t stream) {
         a.C % kUnit ? norm_fwd_pick<T, S, JOIN, 2>(s, run) : norm_fwd_pick<T, S, JOIN, 0>(s, run);
 }
 
-template <typename T, typename S, bool JOIN, int RAGGED, typename Run>
+template <typename T, typename S, bool JOIN, bool SUM, int RAGGED, typename Run>
 void norm_bwd_pick(const NormShape& s, Run run) {
     if (s.threads == 0)
-        s.nv == 1 ? run(k_norm_bwd<T, S, JOIN, 1, 0, RAGGED ? 1 : 0>) : run(k_norm_bwd<T, S, JOIN, 2, 0, RAGGED>);
+        s.nv == 1 ? run(k_norm_bwd<T, S, JOIN, 1, 0, RAGGED ? 1 : 0, SUM>) : run(k_norm_bwd<T, S, JOIN, 2, 0, RAGGED, SUM>);
     else if (s.threads == 256)
-        s.nv == 1 ? run(k_norm_bwd<T, S, JOIN, 1, 256, RAGGED>) : run(k_norm_bwd<T, S, JOIN, 2, 256, RAGGED>);
+        s.nv == 1 ? run(k_norm_bwd<T, S, JOIN, 1, 256, RAGGED, SUM>) : run(k_norm_bwd<T, S, JOIN, 2, 256, RAGGED, SUM>);
     else
-        run(k_norm_bwd<T, S, JOIN, 2, 512, RAGGED>);
+        run(k_norm_bwd<T, S, JOIN, 2, 512, RAGGED, SUM>);
 }
-template <typename T, typename S, bool JOIN>
+template <typename T, typename S, bool JOIN, bool SUM = false>
 void norm_bwd_launch(NormBwdArgs a, hipStream_t stream) {
     typedef typename std::conditional<JOIN, S, T>::type H;
     const NormShape s = norm_shape(a.C);
@@ -589,18 +630,18 @@ void norm_bwd_launch(NormBwdArgs a, hipStream_t stream) {
     if (!sums) a.partial = nullptr;
     if (s.nv == 0) {
         const int units = (a.C + kUnit - 1) / kUnit, most = 2 * row_ops_cus();
-        hipLaunchKernelGGL((k_norm_bwd_long<T, S, JOIN>), dim3(a.rows < most ? a.rows : most), dim3(1024), 0, stream, a);
+        hipLaunchKernelGGL((k_norm_bwd_long<T, S, JOIN, SUM>), dim3(a.rows < most ? a.rows : most), dim3(1024), 0, stream, a);
         if (!sums) return;
-        hipLaunchKernelGGL((k_norm_bwd_cols_long<T, H>), dim3(ceil_div(units, 256), blocks), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_norm_bwd_cols_long<T, H, SUM>), dim3(ceil_div(units, 256), blocks), dim3(256), 0, stream, a);
         norm_finish(a, blocks, stream);
         return;
     }
     const dim3 grid(blocks), block(s.block());
     const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a); };
     if (a.C < kUnit)
-        run(k_norm_bwd<T, S, JOIN, 1, 0, 3>);
+        run(k_norm_bwd<T, S, JOIN, 1, 0, 3, SUM>);
     else
-        a.C % kUnit ? norm_bwd_pick<T, S, JOIN, 2>(s, run) : norm_bwd_pick<T, S, JOIN, 0>(s, run);
+        a.C % kUnit ? norm_bwd_pick<T, S, JOIN, SUM, 2>(s, run) : norm_bwd_pick<T, S, JOIN, SUM, 0>(s, run);
     if (sums && blocks > 1) norm_finish(a, blocks, stream);
 }
 

@@ -31,6 +31,8 @@ struct Entries {
     decltype(&fiery_dropout) dropout;
     decltype(&fiery_dropout_add_layer_norm_fwd) join_fwd;
     decltype(&fiery_dropout_add_layer_norm_bwd) join_bwd;
+    decltype(&fiery_dropout_add_layer_norm_fwd_unrounded) join_fwd_unrounded;
+    decltype(&fiery_dropout_add_layer_norm_bwd_unrounded) join_bwd_unrounded;
 };
 
 // where a call goes
@@ -249,37 +251,43 @@ struct Dropout : torch::autograd::Function<Dropout> {
 int64_t* used_behind(const Tensor& stats, int64_t rows) { return reinterpret_cast<int64_t*>(floats(stats, 2 * rows)); }
 
 variable_list join_forward(const Tensor& x, const Tensor& residual, const Tensor& weight, const Tensor& bias, const Tensor& rng, const Mask& m, int64_t call,
-                           double eps, const To& to, const Tensor& stats) {
+                           double eps, bool of_sum, const To& to, const Tensor& stats) {
     const Sizes s = sizes_of(x);
     Tensor y = dense_like(x, x.scalar_type()), h = dense_like(x, residual.scalar_type());
     if (s.rows) {
         const auto [xr, ld] = rows_of(x);
         const auto [rr, r_ld] = rows_of(residual);
         const Tensor& params = weight.defined() ? weight : bias;
-        check(to, to.lib->join_fwd(ptr(xr), ld, type_of(xr), ptr(rr), r_ld, type_of(rr), s.rows, static_cast<int>(s.c), ptr(weight), ptr(bias),
-                                   params.defined() ? type_of(params) : 0, static_cast<float>(eps), static_cast<int>(m.threshold),
-                                   m.threshold ? numbers(rng) : nullptr, call, m.share, static_cast<int>(m.one_column), used_behind(stats, s.rows), ptr(y), s.c, ptr(h), s.c,
-                                   floats(stats), floats(stats, s.rows), to.stream));
+        const auto call_fwd = of_sum ? to.lib->join_fwd_unrounded : to.lib->join_fwd;
+        check(to, call_fwd(ptr(xr), ld, type_of(xr), ptr(rr), r_ld, type_of(rr), s.rows, static_cast<int>(s.c), ptr(weight), ptr(bias),
+                           params.defined() ? type_of(params) : 0, static_cast<float>(eps), static_cast<int>(m.threshold),
+                           m.threshold ? numbers(rng) : nullptr, call, m.share, static_cast<int>(m.one_column), used_behind(stats, s.rows), ptr(y), s.c, ptr(h), s.c,
+                           floats(stats), floats(stats, s.rows), to.stream));
     }
     return {y, h};
 }
 
 struct DropoutAddLayerNorm : torch::autograd::Function<DropoutAddLayerNorm> {
+    // inputs: the backward pass reads x and the residual, not h (an h of 32 bits is not rounded: then it reads that)
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const Maybe& weight_, const Maybe& bias_, const Maybe& rng,
-                                 int64_t threshold, int64_t share, int64_t one_column, int64_t call, double eps, int64_t entries, int64_t stream) {
+                                 int64_t threshold, int64_t share, int64_t one_column, int64_t call, double eps, bool inputs, int64_t entries, int64_t stream) {
         const Tensor weight = or_none(weight_), bias = or_none(bias_);
         const Mask m{threshold, share, one_column};
         const Tensor stats = at::empty({2 * sizes_of(x).rows + 4}, x.options().dtype(at::kFloat).requires_grad(false));
-        variable_list out = join_forward(x, residual, weight, bias, or_none(rng), m, call, eps, to_of(entries, stream), stats);
+        const bool of_sum = inputs && residual.scalar_type() != at::kFloat;
+        const auto [xr, x_ld] = of_sum ? rows_of(x) : std::pair<Tensor, int64_t>(x, 0);
+        const auto [rr, r_ld] = of_sum ? rows_of(residual) : std::pair<Tensor, int64_t>(residual, 0);
+        variable_list out = join_forward(xr, rr, weight, bias, or_none(rng), m, call, eps, of_sum, to_of(entries, stream), stats);
         ctx->set_materialize_grads(false);
-        ctx->save_for_backward({out[1], weight, stats});
-        ctx->saved_data[kMeta] = std::vector<int64_t>{static_cast<int64_t>(x.scalar_type()), type_or_none(bias), threshold, share, one_column, entries, stream};
+        ctx->save_for_backward({of_sum ? rr : out[1], weight, stats, of_sum ? xr : Tensor()});
+        ctx->saved_data[kMeta] = std::vector<int64_t>{static_cast<int64_t>(x.scalar_type()), type_or_none(bias), threshold, share, one_column, entries, stream,
+                                                      of_sum ? r_ld : sizes_of(x).c, x_ld};
         return out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list incoming) {
         const variable_list saved = ctx->get_saved_variables();
         return once(incoming, saved, [&]() -> variable_list {
-            const Tensor &h = saved[0], &weight = saved[1], &stats = saved[2];
+            const Tensor &h = saved[0], &weight = saved[1], &stats = saved[2], &x = saved[3];              // (x: then h is the residual)
             const auto meta = ctx->saved_data[kMeta].toIntVector();
             const auto x_type = static_cast<at::ScalarType>(meta[0]);
             const Mask m{meta[2], meta[3], meta[4]};
@@ -302,14 +310,21 @@ struct DropoutAddLayerNorm : torch::autograd::Function<DropoutAddLayerNorm> {
             if (s.rows) {
                 const auto [gr, dy_ld] = rows_of(dy);
                 const auto [hg, dh_ld] = dh.defined() ? rows_of(dh) : std::pair<Tensor, int64_t>();
-                check(to, to.lib->join_bwd(ptr(gr), dy_ld, ptr(hg), dh_ld, ptr(h), s.c, type_of(x_type), type_of(h), s.rows, static_cast<int>(s.c), ptr(weight),
-                                           weight.defined() ? type_of(weight) : p.type, floats(stats), floats(stats, s.rows), static_cast<int>(m.threshold),
-                                           used, m.share, static_cast<int>(m.one_column), ptr(dx), s.c, ptr(dr), s.c, ptr(p.dw), ptr(p.db),
-                                           floats(p.workspace), p.floats, to.stream));
+                const int param_type = weight.defined() ? type_of(weight) : p.type;
+                if (x.defined())
+                    check(to, to.lib->join_bwd_unrounded(ptr(gr), dy_ld, ptr(hg), dh_ld, ptr(x), meta[8], ptr(h), meta[7], type_of(h), s.rows, static_cast<int>(s.c),
+                                                         ptr(weight), param_type, floats(stats), floats(stats, s.rows), static_cast<int>(m.threshold), used,
+                                                         m.share, static_cast<int>(m.one_column), ptr(dx), s.c, ptr(dr), s.c, ptr(p.dw), ptr(p.db),
+                                                         floats(p.workspace), p.floats, to.stream));
+                else
+                    check(to, to.lib->join_bwd(ptr(gr), dy_ld, ptr(hg), dh_ld, ptr(h), meta[7], type_of(x_type), type_of(h), s.rows, static_cast<int>(s.c), ptr(weight),
+                                               param_type, floats(stats), floats(stats, s.rows), static_cast<int>(m.threshold), used, m.share,
+                                               static_cast<int>(m.one_column), ptr(dx), s.c, ptr(dr), s.c, ptr(p.dw), ptr(p.db), floats(p.workspace), p.floats,
+                                               to.stream));
             } else {
                 p.zero();
             }
-            return {dx, dr, p.dw, p.db, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+            return {dx, dr, p.dw, p.db, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
         });
     }
 };
@@ -336,15 +351,16 @@ Tensor dropout(const Tensor& x, const Maybe& residual, const Maybe& rng, const s
 }
 
 std::pair<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const Tensor& residual, const Maybe& weight, const Maybe& bias, const Maybe& rng,
-                                                 const std::tuple<int64_t, int64_t, int64_t>& mask, int64_t call, double eps, int64_t entries, int64_t stream) {
+                                                 const std::tuple<int64_t, int64_t, int64_t>& mask, int64_t call, double eps, bool inputs, int64_t entries,
+                                                 int64_t stream) {
     const OnDevice on(x);
     const Tensor w = dense(weight), b = dense(bias);
     const auto [threshold, share, one_column] = mask;
     variable_list out;
     if (at::GradMode::is_enabled() && (wants(x) || wants(residual) || wants(w) || wants(b)))
-        out = DropoutAddLayerNorm::apply(x, residual, maybe(w), maybe(b), rng, threshold, share, one_column, call, eps, entries, stream);
+        out = DropoutAddLayerNorm::apply(x, residual, maybe(w), maybe(b), rng, threshold, share, one_column, call, eps, inputs, entries, stream);
     else
-        out = join_forward(x, residual, w, b, or_none(rng), {threshold, share, one_column}, call, eps, to_of(entries, stream), Tensor());
+        out = join_forward(x, residual, w, b, or_none(rng), {threshold, share, one_column}, call, eps, false, to_of(entries, stream), Tensor());
     return {out[0], out[1]};
 }
 

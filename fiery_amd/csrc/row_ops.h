@@ -269,21 +269,47 @@ __device__ __forceinline__ uint4 philox(unsigned c0, unsigned c1, unsigned c2, u
     r.w = c3;
     return r;
 }
-// One unit of a row.  (A select and not a product: a dropped infinity or NaN leaves a zero.  Each half is compared in the upper
-// half of a word, with 65536 threshold - 1: 2^32 - 1 where everything is dropped.)
-__device__ __forceinline__ void drop_unit(const DropArgs& d, const DropKey& k, unsigned row, unsigned unit, float (&v)[kUnit]) {
-    if (d.threshold == 0) return;
+// The words of one unit of a row.
+__device__ __forceinline__ uint4 drop_words(const DropArgs& d, const DropKey& k, unsigned row, unsigned unit) {
     const unsigned mask_row = d.rows_per_mask.d > 1 ? div_by(row, d.rows_per_mask) : row;
     uint4 w = philox(d.one_column ? 0u : unit, mask_row, k.call_lo, k.call_hi, k.seed_lo, k.seed_hi);
     if (d.one_column) {
         w.x = (w.x << 16) | (w.x & 0xffffu);
         w.y = w.z = w.w = w.x;
     }
+    return w;
+}
+// One unit of a row.  (A select and not a product: a dropped infinity or NaN leaves a zero.  Each half is compared in the upper
+// half of a word, with 65536 threshold - 1: 2^32 - 1 where everything is dropped.)
+__device__ __forceinline__ void drop_unit(const DropArgs& d, const DropKey& k, unsigned row, unsigned unit, float (&v)[kUnit]) {
+    if (d.threshold == 0) return;
+    const uint4 w = drop_words(d, k, row, unit);
     const unsigned word[4] = {w.x, w.y, w.z, w.w}, limit = d.threshold * 65536u - 1u;
 #pragma unroll
     for (int j = 0; j < kUnit; ++j) v[j] = (j & 1 ? word[j / 2] : word[j / 2] << 16) > limit ? v[j] * d.scale : 0.f;
 }
-
+// The same in two steps, for a mask that is used twice (threshold > 0): bit j is set where column j is kept.
+__device__ __forceinline__ unsigned drop_bits(const DropArgs& d, const DropKey& k, unsigned row, unsigned unit) {
+    const uint4 w = drop_words(d, k, row, unit);
+    const unsigned word[4] = {w.x, w.y, w.z, w.w};
+    unsigned bits = 0;
+#pragma unroll
+    for (int j = kUnit - 1; j >= 0; --j) {
+        const unsigned half = j & 1 ? word[j / 2] >> 16 : word[j / 2] & 0xffffu;
+        bits = bits + bits + ((d.threshold - 1u - half) >> 31);             // (integers: lane masks fill the scalar registers; 4001 bf16 columns 108 us, not 126)
+    }
+    return bits;
+}
+__device__ __forceinline__ void drop_by(const DropArgs& d, unsigned bits, float (&v)[kUnit]) {
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j) {
+        unsigned u;
+        const float scaled = v[j] * d.scale;
+        __builtin_memcpy(&u, &scaled, 4);
+        u &= 0u - (bits >> j & 1u);
+        __builtin_memcpy(&v[j], &u, 4);
+    }
+}
 // host side: the arguments of one call, or an error text
 inline const char* drop_args(DropArgs& d, const void* rng, void* rng_used, int64_t call, int threshold, int64_t rows_per_mask, int one_column) {
     if (threshold < 0 || threshold > 65536) return "threshold outside 0 .. 65536";

@@ -13,7 +13,7 @@ import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'libfiery_hip.so')
-ABI_VERSION = 26
+ABI_VERSION = 27
 
 c_float_p = C.POINTER(C.c_float)
 c_int32_p = C.POINTER(C.c_int32)
@@ -185,6 +185,10 @@ _SIGNATURES = {
                                                    C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_int,
                                                    C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
                                                    C.c_void_p]),
+    'fiery_dropout_add_layer_norm_bwd_unrounded': (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                                             C.c_int, C.c_int64, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p,
+                                                             C.c_int64, C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p,
+                                                             C.c_void_p, C.c_int64, C.c_void_p]),
     'fiery_gru_reset_fwd': (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_int,
                                       C.c_void_p]),
     'fiery_gru_reset_bwd': (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_int,
@@ -215,11 +219,14 @@ _SIGNATURES = {
     'fiery_nhwc_to_nchw': (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]),
 }
 
+_SIGNATURES['fiery_dropout_add_layer_norm_fwd_unrounded'] = _SIGNATURES['fiery_dropout_add_layer_norm_fwd']
+
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 
 # what csrc/row_autograd.cpp calls, in the order of its `Entries`
 ROW_ENTRIES = ('fiery_last_error', 'fiery_layer_norm_fwd', 'fiery_layer_norm_bwd_workspace_floats', 'fiery_layer_norm_bwd', 'fiery_dropout',
-               'fiery_dropout_add_layer_norm_fwd', 'fiery_dropout_add_layer_norm_bwd')
+               'fiery_dropout_add_layer_norm_fwd', 'fiery_dropout_add_layer_norm_bwd', 'fiery_dropout_add_layer_norm_fwd_unrounded',
+               'fiery_dropout_add_layer_norm_bwd_unrounded')
 
 
 def require_usable_gpu_process(what):

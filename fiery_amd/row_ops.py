@@ -140,12 +140,19 @@ def dropout(x, p, rng=None, *, call=0, per='element', residual=None, lib=None):
     return _autograd().dropout(x, residual, rng if mask[0] else None, mask, call, entries, stream)
 
 
-def dropout_add_layer_norm(x, residual, weight=None, bias=None, p=0.0, rng=None, *, call=0, per='element', eps=1e-5, lib=None):
+def dropout_add_layer_norm(x, residual, weight=None, bias=None, p=0.0, rng=None, *, call=0, per='element', eps=1e-5, keep='h', lib=None):
     """h = residual + dropout(x, p), y = layer_norm(h, weight, bias) in one pass each way -> (y, h): y in x's type, h in the residual's
-    (float32 or x's type).  y comes from h before it is rounded to that type; the gradients are the norm's at the h that is returned."""
+    (float32 or x's type).  y comes from h before it is rounded to that type.
+
+    keep: what the backward pass reads where h has 16 bits.  'h' - the h that is returned: the gradients are the norm's at that h, and the
+    weight's carries its rounding (more of it the larger a row's mean is beside its spread; no finite gradient where h overflows fp16).
+    'inputs' - x and residual, which autograd then keeps: h is made again before its rounding, the gradients are as exact as beside an h
+    of 32 bits, and the pass reads one tensor more.  An h of 32 bits is not rounded: the two are the same there."""
+    if keep not in ('h', 'inputs'):
+        raise ValueError(f"dropout_add_layer_norm: keep is 'h' or 'inputs', got {keep!r}")
     _check_x(x, 'dropout_add_layer_norm')
     _check_residual(x, residual, 'dropout_add_layer_norm')
     _check_params(x, weight, bias, 'dropout_add_layer_norm')
     mask = _mask_args(x, p, rng, call, per, 'dropout_add_layer_norm')
     entries, stream = _to(lib, x)
-    return _autograd().dropout_add_layer_norm(x, residual, weight, bias, rng if mask[0] else None, mask, call, eps, entries, stream)
+    return _autograd().dropout_add_layer_norm(x, residual, weight, bias, rng if mask[0] else None, mask, call, eps, keep == 'inputs', entries, stream)

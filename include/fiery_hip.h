@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define FIERY_ABI_VERSION 26      /* 26: row operators (fiery_layer_norm_*, fiery_dropout, fiery_dropout_add_layer_norm_*); 25 (round 6): fiery_conv_desc grew (weights2_split, weights3_split); 24 (round 6): the split Winograd form (fiery_conv_pack_weights_winograd_split, FIERY_CONV_FORM_WINOGRAD_SPLIT); 23 (round 6): fiery_conv_form_used, FIERY_POOL_NO_RANKS, the prepass quantises without divisions where that is exact; 22 (round 5): fiery_conv_desc grew (weights_winograd, winograd, stream_k, sk_*); fiery_conv_pack_weights_winograd, fiery_conv_winograd_packed_floats, fiery_conv_stream_k_plan */
+#define FIERY_ABI_VERSION 27      /* 27: fiery_dropout_add_layer_norm_fwd_unrounded / _bwd_unrounded; 26: row operators (fiery_layer_norm_*, fiery_dropout, fiery_dropout_add_layer_norm_*); 25 (round 6): fiery_conv_desc grew (weights2_split, weights3_split); 24 (round 6): the split Winograd form (fiery_conv_pack_weights_winograd_split, FIERY_CONV_FORM_WINOGRAD_SPLIT); 23 (round 6): fiery_conv_form_used, FIERY_POOL_NO_RANKS, the prepass quantises without divisions where that is exact; 22 (round 5): fiery_conv_desc grew (weights_winograd, winograd, stream_k, sk_*); fiery_conv_pack_weights_winograd, fiery_conv_winograd_packed_floats, fiery_conv_stream_k_plan */
 
 #define FIERY_OK 0
 #define FIERY_EINVAL (-22)      /* bad argument (shape, alignment, null pointer) */
@@ -597,6 +597,19 @@ int fiery_dropout_add_layer_norm_bwd(const void* dy, int64_t dy_ld, const void* 
                                      const float* rstd, int threshold, const int64_t* rng_used, int64_t rows_per_mask, int one_column,
                                      void* dx, int64_t dx_ld, void* dresidual, int64_t dres_ld, void* dgamma, void* dbeta, float* workspace,
                                      int64_t workspace_floats, fiery_stream_t stream);
+
+/* The same pair with the gradient at the h before its rounding, for a stream of 16 bits: _fwd_unrounded leaves the mean and rstd of that
+ * h (its other results are those of _fwd), _bwd_unrounded reads x and residual (both of `type`, bf16 or fp16) in place of h and makes it
+ * again.  dgamma then carries no rounding of h, and a row whose h overflows fp16 keeps finite gradients; one tensor more is read. */
+int fiery_dropout_add_layer_norm_fwd_unrounded(const void* x, int64_t x_ld, int x_type, const void* residual, int64_t res_ld, int stream_type,
+                                               int64_t rows, int C, const void* gamma, const void* beta, int param_type, float eps, int threshold,
+                                               const int64_t* rng, int64_t call, int64_t rows_per_mask, int one_column, int64_t* rng_used, void* y,
+                                               int64_t y_ld, void* h, int64_t h_ld, float* mean, float* rstd, fiery_stream_t stream);
+int fiery_dropout_add_layer_norm_bwd_unrounded(const void* dy, int64_t dy_ld, const void* dh, int64_t dh_ld, const void* x, int64_t x_ld,
+                                               const void* residual, int64_t res_ld, int type, int64_t rows, int C, const void* gamma, int param_type,
+                                               const float* mean, const float* rstd, int threshold, const int64_t* rng_used, int64_t rows_per_mask,
+                                               int one_column, void* dx, int64_t dx_ld, void* dresidual, int64_t dres_ld, void* dgamma, void* dbeta,
+                                               float* workspace, int64_t workspace_floats, fiery_stream_t stream);
 
 /* BatchNorm with batch statistics (+ fused ReLU) on pixel-major rows - what `nn.BatchNorm2d / BatchNorm3d (+ nn.ReLU)` of the
  * BEV stack compute in train() mode (layers/convolutions.py:27-34, 85-105; layers/temporal.py:77-84, 107-117; autograd's

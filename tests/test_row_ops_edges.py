@@ -1,0 +1,131 @@
+"""Row operators at their edges: gradients at an h that is stored in 16 bits, and calls whose answers once were wrong.  Definitions and
+bounds are those of tests/test_row_ops.py."""
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from fiery_amd import native, row_ops
+from tests.test_row_ops import BF16, F16, F32, U, Backend, check_norm_forward, check_stored, depth, kept, make, norm64, on, skip_long, xhat_error  # noqa: F401
+
+
+# ---- gradients of the joined operator at the h before its rounding -----------------------------------------------------------
+def grads_near(dy, h, off, weight, eps, dh):
+    """64-bit gradients at h and the bounds of 32-bit ones whose h is up to `off` away, as test_row_ops.norm_grads.  What off adds, to
+    first order: a row's rstd moves by rstd^2 mean(|xhat| (off + mean off)), which xhat and the gradient are multiples of."""
+    mean, rstd, xhat = norm64(h, weight, None, eps)
+    w = weight.double().cpu()
+    moved = rstd * (xhat.abs() * (off + off.mean(-1, keepdim=True))).mean(-1, keepdim=True)
+    d, ex = depth(h.shape[-1]), xhat_error(h, mean, rstd, xhat, off) + xhat.abs() * moved
+    gg = dy * w
+    m1, m2 = gg.mean(-1, keepdim=True), (gg * xhat).mean(-1, keepdim=True)
+    e1 = (d + 2) * U * gg.abs().mean(-1, keepdim=True)
+    e2 = (d + 3) * U * (gg * xhat).abs().mean(-1, keepdim=True) + (gg.abs() * ex).mean(-1, keepdim=True)
+    norm = rstd * (gg - (m1 + xhat * m2))
+    tol = rstd * (2 * U * gg.abs() + e1 + xhat.abs() * e2 + ex * m2.abs() + 4 * U * (m1.abs() + (xhat * m2).abs())) + ((d / 2 + 8) * U + moved) * norm.abs()
+    if dh is not None:
+        norm = norm + dh
+        tol = tol + 2 * U * (norm.abs() + dh.abs())
+    lead = tuple(range(h.dim() - 1))
+    rows = h.numel() // h.shape[-1]
+    dw, db = (dy * xhat).sum(lead), dy.sum(lead)
+    return (norm, tol), (dw, (dy.abs() * ex).sum(lead) + (rows + 4) * U * (dy * xhat).abs().sum(lead)), (db, (rows + 4) * U * dy.abs().sum(lead))
+
+
+def join_case(on, shape, dtype, params, seed=30, shift=0.5, pad=0):  # noqa: F811
+    x, r = make(shape, dtype, on.device, seed, 1.5, pad=pad).requires_grad_(), make(shape, dtype, on.device, seed + 1, 1.0, shift, pad=pad).requires_grad_()
+    w, b = make(shape[-1:], params, on.device, seed + 2, 0.3, 1.0).requires_grad_(), make(shape[-1:], params, on.device, seed + 3, 0.3).requires_grad_()
+    return x, r, w, b, make(shape, dtype, on.device, seed + 4), make(shape, dtype, on.device, seed + 5)
+
+
+@pytest.mark.parametrize('per,p', [('element', 0.3), ('channel', 0.3), ('sample', 0.3), ('element', 0.0)])
+@pytest.mark.parametrize('shape,shift,pad', [((1, 1), 0.5, 0), ((3, 7), 0.5, 3), ((4, 5, 35), 0.5, 0), ((9, 64), 60.0, 8), ((2, 3, 200), 20.0, 1), ((40, 3, 24), 0.5, 0),
+                                             ((2, 1000), 0.5, 5), ((3, 2049), 0.5, 0), ((1, 8201), 0.5, 0), ((2, 16400), 0.5, 0)], ids=str)
+@pytest.mark.parametrize('dtype,params', [(BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)], ids=str)
+def test_gradients_at_the_unrounded_sum(on, per, p, shape, shift, pad, dtype, params):  # noqa: F811
+    """keep='inputs': dweight and the others are those of the h that y comes from, at 32-bit accuracy, however far the rows' mean is from
+    zero; y and h are what they are with keep='h'."""
+    skip_long(on, shape[-1] > 8201 or shape[-1] > 2000 and (per != 'element' or dtype is not BF16 or params is not F32))
+    seed, eps = 1 << 50, 1e-3
+    rng = row_ops.dropout_rng(seed, on.device)
+    x, r, w, b, dy, dh = join_case(on, shape, dtype, params, shift=shift, pad=pad)
+    call = lambda keep: row_ops.dropout_add_layer_norm(x, r, w, b, p, rng, call=3, per=per, eps=eps, keep=keep, lib=on.lib)
+    y, h = call('inputs')
+    other = call('h')
+    assert torch.equal(y, other[0]) and torch.equal(h, other[1])
+    m = kept(shape, p, seed, 3, per)
+    dropped = x.detach().double().cpu() * m
+    h64 = dropped + r.detach().double().cpu()
+    off = 3 * U * (dropped.abs() + h64.abs())
+    rng[1] += 17
+    g64, dh64 = dy.double().cpu(), dh.double().cpu()
+    total, gw, gb = grads_near(g64, h64, off, w.detach(), eps, dh64)
+    dx, dr, dw, db = torch.autograd.grad((y, h), (x, r, w, b), (dy, dh), retain_graph=True)
+    check_stored(dr, total)
+    check_stored(dx, (total[0] * m, total[1] * m + 2 * U * (total[0] * m).abs()))
+    check_stored(dw, gw)
+    check_stored(db, gb)
+    only_y, _, _ = grads_near(g64, h64, off, w.detach(), eps, None)
+    check_stored(torch.autograd.grad(y, r, dy, retain_graph=True)[0], only_y)
+    check_stored(torch.autograd.grad(y, w, dy, retain_graph=True)[0], gw)
+    dx, dr = torch.autograd.grad(h, (x, r), dh, retain_graph=True)
+    assert torch.equal(dr, dh)
+    check_stored(dx, (dh64 * m, 2 * U * (dh64 * m).abs()))
+
+
+def test_a_sum_past_the_largest_16_bit_value_keeps_its_gradients(on):  # noqa: F811
+    """60,000 + 60,000 is infinite in fp16: y is finite, and so are the gradients of keep='inputs'."""
+    x, r, w, b, dy, _ = join_case(on, (4, 40), F16, F32)
+    with torch.no_grad():
+        x[1], r[1] = 60000.0, 60000.0
+        r[1, ::2] = 40000.0
+    y, h = row_ops.dropout_add_layer_norm(x, r, w, b, keep='inputs', lib=on.lib)
+    assert torch.isinf(h[1, 1]) and torch.isfinite(y).all()
+    h64 = x.detach().double().cpu() + r.detach().double().cpu()
+    total, gw, gb = grads_near(dy.double().cpu(), h64, 2 * U * h64.abs(), w.detach(), 1e-5, None)
+    dx, dr, dw, db = torch.autograd.grad(y, (x, r, w, b), dy)
+    check_stored(dx, total)
+    check_stored(dr, total)
+    check_stored(dw, gw)
+    check_stored(db, gb)
+
+
+def test_a_32_bit_stream_is_the_same_either_way(on):  # noqa: F811
+    for dtype in (F32, BF16, F16):
+        x, r = make((5, 70), dtype, on.device, 50).requires_grad_(), make((5, 70), F32, on.device, 51).requires_grad_()
+        w, dy = make((70,), F32, on.device, 52, 0.2, 1.0).requires_grad_(), make((5, 70), dtype, on.device, 53)
+        rng = row_ops.dropout_rng(9, on.device)
+        got = []
+        for keep in ('h', 'inputs'):
+            y, h = row_ops.dropout_add_layer_norm(x, r, w, None, 0.4, rng, keep=keep, lib=on.lib)
+            got.append([y, h, *torch.autograd.grad(y, (x, r, w), dy)])
+        assert all(torch.equal(p, q) for p, q in zip(*got))
+
+
+def test_what_is_kept_and_refused(sim):
+    """keep='inputs' notices a changed input; other words and entry points without a 16-bit stream are refused."""
+    x, r = torch.ones(3, 16, dtype=BF16).requires_grad_(), torch.ones(3, 16, dtype=BF16)
+    z = x * 2.0
+    y, h = row_ops.dropout_add_layer_norm(z, r, keep='inputs', lib=sim)
+    h += 1.0                                                       # h is no longer what the backward pass reads
+    torch.autograd.grad(y.float().sum(), x, retain_graph=True)
+    z += 1.0
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.float().sum().backward()
+    with pytest.raises(ValueError, match='keep'):
+        row_ops.dropout_add_layer_norm(x, r, keep='x', lib=sim)
+    p = torch.zeros(64).data_ptr()
+    bwd = lambda x=p, res=p, t=1, x_ld=8: sim.check(sim.dll.fiery_dropout_add_layer_norm_bwd_unrounded(
+        p, 8, None, 0, x, x_ld, res, 8, t, 2, 8, p, t, p, p, 0, None, 1, 0, p, 8, p, 8, None, None, None, 0, None))
+    for kw in (dict(x=None), dict(res=None), dict(t=0), dict(t=3), dict(x_ld=-1)):
+        with pytest.raises(native.NativeError):
+            bwd(**kw)
+
+
+@pytest.mark.parametrize('where', ['end', 'begin'])
+def test_the_unrounded_kernels_stay_inside_their_operands(sim, where):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    res = subprocess.run([sys.executable, os.path.join(root, 'tests', 'sim', 'guard_unrounded.py'), where], cwd=root, capture_output=True, text=True, timeout=900)
+    assert res.returncode == 0 and f'ok unrounded {where} (' in res.stdout, res.stdout[-1500:] + res.stderr[-3000:]
