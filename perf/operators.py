@@ -176,7 +176,8 @@ def _calls(s):
             return {'y': y, 'dx': torch.autograd.grad(y, x, s['dy'])[0]}
         dx, dr = torch.autograd.grad(y, (x, residual), s['dy'])
         return {'y': y, 'dx': dx, 'dresidual': dr}
-    y, h = row_ops.dropout_add_layer_norm(x, s['residual'], s['weight'], s['bias'], case['p'], s['rng'], per=case['per'], eps=EPS)
+    # (gradients at h before its rounding, as the definition has them)
+    y, h = row_ops.dropout_add_layer_norm(x, s['residual'], s['weight'], s['bias'], case['p'], s['rng'], per=case['per'], eps=EPS, keep='inputs')
     if not case['train']:
         return {'y': y, 'h': h}
     dx, dr, dw, db = torch.autograd.grad((y, h), (x, s['residual'], s['weight'], s['bias']), (s['dy'], s['dh']))
