@@ -57,6 +57,9 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {
     return v;
 }
 
+// whether it holds in any lane of the wavefront
+__device__ __forceinline__ bool any_lane(bool p) { return __builtin_amdgcn_ballot_w64(p) != 0; }
+
 // v_rsq_f32: 1 / sqrt(x) to about an ulp, for x well inside the range of normal numbers
 __device__ __forceinline__ float rsq_estimate(float x) { return __builtin_amdgcn_rsqf(x); }
 // the low word of (hi:lo) >> (16 * halves), halves 0 or 1

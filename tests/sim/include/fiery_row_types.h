@@ -37,6 +37,7 @@ inline float lanes_sum(float v, int lanes) {
     for (int m = 1; m < lanes; m <<= 1) v += __shfl_xor(v, m);
     return v;
 }
+inline bool any_lane(bool p) { return lanes_sum(p ? 1.0f : 0.0f, 64) != 0.0f; }
 inline float rsq_estimate(float x) { return 1.0f / std::sqrt(x); }
 inline unsigned funnel_halves(unsigned hi, unsigned lo, unsigned halves) {
     return static_cast<unsigned>(((static_cast<unsigned long long>(hi) << 32) | lo) >> (16 * halves));

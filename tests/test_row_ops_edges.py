@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from fiery_amd import native, row_ops
-from tests.test_row_ops import BF16, F16, F32, U, Backend, check_norm_forward, check_stored, depth, kept, make, norm64, on, skip_long, xhat_error  # noqa: F401
+from tests.test_row_ops import BF16, F16, F32, U, Backend, check_stored, depth, kept, make, norm64, on, skip_long, xhat_error  # noqa: F401
 
 
 # ---- gradients of the joined operator at the h before its rounding -----------------------------------------------------------
@@ -129,3 +129,58 @@ def test_the_unrounded_kernels_stay_inside_their_operands(sim, where):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     res = subprocess.run([sys.executable, os.path.join(root, 'tests', 'sim', 'guard_unrounded.py'), where], cwd=root, capture_output=True, text=True, timeout=900)
     assert res.returncode == 0 and f'ok unrounded {where} (' in res.stdout, res.stdout[-1500:] + res.stderr[-3000:]
+
+
+# ---- means whose sums round ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('c', [1, 3, 8, 72, 300, 513, 1000, 2049, 8200])
+@pytest.mark.parametrize('value', [0.1, -1000.1, 12345.678, 1e30, -1e36])
+def test_a_constant_row_is_its_bias(on, c, value):  # noqa: F811
+    """The sum of equal values is rounded, its mean is not: y is the bias exactly (v - v = 0), and dx is rstd (g - mean g) with
+    rstd = 1 / sqrt(eps), as test_row_ops.norm_grads bounds it; neighbours of ordinary values are what they are without it."""
+    skip_long(on, c > 2049)
+    x = make((5, c), F32, on.device, 60, 2.0, 0.5)
+    alone = x[[0, 4]].clone()
+    x[1], x[3] = value, value
+    leaf, w, b = x.clone().requires_grad_(), make((c,), F32, on.device, 61, 0.2, 1.0), make((c,), F32, on.device, 62)
+    dy = make((5, c), F32, on.device, 63)
+    y = row_ops.layer_norm(leaf, w, b, lib=on.lib)
+    assert torch.equal(y[1], b) and torch.equal(y[3], b)
+    assert torch.equal(y[[0, 4]], row_ops.layer_norm(alone, w, b, lib=on.lib))
+    dx, = torch.autograd.grad(y, leaf, dy)
+    g = dy[[1, 3]].double().cpu() * w.double().cpu()
+    want = (g - g.mean(-1, keepdim=True)) / 1e-5 ** 0.5
+    # xhat is 0: rstd's own error (3 u), the row mean's (DEPTH + 2) u, the products'
+    tol = ((depth(c) + 2) * U * g.abs().mean(-1, keepdim=True) + 4 * U * g.abs()) / 1e-5 ** 0.5 + 8 * U * want.abs()
+    check_stored(dx[[1, 3]], (want, tol))
+
+
+@pytest.mark.parametrize('c', [24, 72, 1000])
+@pytest.mark.parametrize('dtype,stream', [(F32, F32), (BF16, BF16), (F16, F16), (F16, F32)], ids=str)
+def test_a_constant_sum_is_its_bias(on, c, dtype, stream):  # noqa: F811
+    """The joined operator's statistics, both those of y and those that are kept: constant rows have xhat 0 in each."""
+    value = 1000.1 if dtype is F32 else 12.3
+    x, r = make((4, c), dtype, on.device, 64), make((4, c), stream, on.device, 65)
+    x[2], r[2] = value, value / 3
+    x, r, b = x.requires_grad_(), r.requires_grad_(), make((c,), dtype, on.device, 66)
+    w = torch.ones(c, dtype=dtype, device=on.device, requires_grad=True)
+    for keep in ('h', 'inputs'):
+        y, h = row_ops.dropout_add_layer_norm(x, r, w, b, keep=keep, lib=on.lib)
+        assert torch.equal(y[2], b)
+        dy = torch.zeros(4, c, dtype=dtype, device=on.device)
+        dy[2] = 1.0
+        dx, dw = torch.autograd.grad(y, (x, w), dy)
+        assert not dw.any()                                        # dy xhat, xhat 0
+        assert not dx[[0, 1, 3]].any()
+        # (g - mean g) of equal g: the mean's rounding, (DEPTH + 2) u, over sqrt(eps); and its own rounding when it is stored
+        assert float(dx[2].abs().max()) <= (depth(c) + 2) * U / 1e-5 ** 0.5 * 1.01
+
+
+def test_a_mean_far_above_the_spread(on):  # noqa: F811
+    """One value of c is a step (2^-10) above the others, 12345.678: the mean lies a c-th of a step above them and is rounded to them, so
+    values are off by step / c, and the variance, (1 - 1/c) / c steps^2, by its c-th at most."""
+    for c in (72, 513, 1000):
+        x = torch.full((1, c), 12345.678, device=on.device)
+        x[0, 5] += 2.0 ** -10
+        y = row_ops.layer_norm(x, None, None, 1e-12, lib=on.lib).double().cpu()
+        mean, rstd, xhat = norm64(x.double().cpu(), None, None, 1e-12)
+        assert ((y - xhat).abs() <= 1.01 * (rstd * 2.0 ** -10 / c + xhat.abs() / c)).all(), c
