@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <initializer_list>
 #include <optional>
 #include <stdexcept>
 #include <utility>
@@ -329,6 +330,13 @@ struct DropoutAddLayerNorm : torch::autograd::Function<DropoutAddLayerNorm> {
     }
 };
 
+// What the operators do not provide is an error.  (A dual tensor without a gradient would go past the nodes and lose its tangent.)
+void provided(std::initializer_list<const Tensor*> operands) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor* t : operands)
+        if (t->defined() && t->_fw_grad(0).defined()) throw std::runtime_error("row operators: forward-mode derivatives are not provided");
+}
+
 // ---- what Python calls, with arguments that it has checked ------------------------------------------------------------------------
 Tensor dense(const Maybe& t) { return t.has_value() ? t->contiguous() : Tensor(); }
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
@@ -336,6 +344,7 @@ bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 Tensor layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, double eps, int64_t entries, int64_t stream) {
     const OnDevice on(x);
     const Tensor w = dense(weight), b = dense(bias);
+    provided({&x, &w, &b});
     if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b))) return LayerNorm::apply(x, maybe(w), maybe(b), eps, entries, stream);
     const auto [xr, ld] = rows_of(x);
     return norm_forward(xr, ld, w, b, eps, to_of(entries, stream), Tensor());
@@ -345,6 +354,7 @@ Tensor dropout(const Tensor& x, const Maybe& residual, const Maybe& rng, const s
                int64_t stream) {
     const OnDevice on(x);
     const Tensor r = or_none(residual);
+    provided({&x, &r});
     const auto [threshold, share, one_column] = mask;
     if (at::GradMode::is_enabled() && (wants(x) || wants(r))) return Dropout::apply(x, residual, rng, threshold, share, one_column, call, entries, stream);
     return drop(x, r, r.defined() ? r.scalar_type() : x.scalar_type(), {threshold, share, one_column}, numbers(or_none(rng)), call, nullptr, to_of(entries, stream));
@@ -355,6 +365,7 @@ std::pair<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const Tensor& 
                                                  int64_t stream) {
     const OnDevice on(x);
     const Tensor w = dense(weight), b = dense(bias);
+    provided({&x, &residual, &w, &b});
     const auto [threshold, share, one_column] = mask;
     variable_list out;
     if (at::GradMode::is_enabled() && (wants(x) || wants(residual) || wants(w) || wants(b)))

@@ -184,3 +184,35 @@ def test_a_mean_far_above_the_spread(on):  # noqa: F811
         y = row_ops.layer_norm(x, None, None, 1e-12, lib=on.lib).double().cpu()
         mean, rstd, xhat = norm64(x.double().cpu(), None, None, 1e-12)
         assert ((y - xhat).abs() <= 1.01 * (rstd * 2.0 ** -10 / c + xhat.abs() / c)).all(), c
+
+
+# ---- calls that the operators do not provide are errors ------------------------------------------------------------------------
+def _ops(lib, rng):
+    """Each operator as a function of one tensor, its other operands plain."""
+    return {'layer_norm': lambda t: row_ops.layer_norm(t, lib=lib), 'dropout': lambda t: row_ops.dropout(t, 0.5, rng, lib=lib),
+            'joined': lambda t: row_ops.dropout_add_layer_norm(t, torch.ones_like(t), p=0.5, rng=rng, lib=lib)[0]}
+
+
+@pytest.mark.parametrize('name', ['layer_norm', 'dropout', 'joined'])
+def test_forward_mode_derivatives_are_refused(sim, name):
+    """A tangent on any operand is an error, with and without a parameter that requires a gradient; it never comes out as zero."""
+    import torch.autograd.forward_ad as fwd
+    rng, x, w = row_ops.dropout_rng(0, 'cpu'), make((4, 16), F32, 'cpu', 70), make((16,), F32, 'cpu', 71)
+    op = _ops(sim, rng)[name]
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        p, learnt = fwd.make_dual(w, torch.ones_like(w)), w.clone().requires_grad_()
+        norm, drop, join = row_ops.layer_norm, row_ops.dropout, row_ops.dropout_add_layer_norm
+        calls = [lambda: op(dual)] + {
+            'layer_norm': [lambda: norm(x, p, w, lib=sim), lambda: norm(x, w, p, lib=sim), lambda: norm(dual, learnt, lib=sim)],
+            'dropout': [lambda: drop(x, 0.5, rng, residual=dual, lib=sim), lambda: drop(dual, 0.5, rng, residual=x.clone().requires_grad_(), lib=sim)],
+            'joined': [lambda: join(x, x, p, w, lib=sim), lambda: join(x, x, w, p, lib=sim), lambda: join(x, dual, lib=sim), lambda: join(x, dual, learnt, lib=sim)],
+        }[name]
+        for call in calls:
+            with pytest.raises(RuntimeError, match='forward-mode'):
+                call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match='forward-mode'):
+            op(dual)                                               # tangents live under no_grad too
+        with fwd._set_fwd_grad_enabled(False):
+            assert torch.equal(op(dual), op(x))                    # nobody asks for one
+        assert torch.equal(op(fwd.unpack_dual(dual).primal), op(x))
