@@ -5,6 +5,8 @@
 // These are the same nodes in C++.  Host code only: the library is reached through the addresses that Python took from it, so the
 // product's and the simulator's builds serve alike, and a node launches on the stream that its forward pass was given, which is
 // the one autograd makes current for the backward pass.
+#include <ATen/TracerMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
@@ -94,10 +96,19 @@ struct Mask {
     int64_t threshold, share, one_column;
 };
 
+// A trace sees the allocation of a result and not the launch that fills it: the traced function would return what the memory held.
+void untraced() {
+    using c10::impl::TorchDispatchModeTLS;
+    if (at::tracer::impl::is_dispatch_enabled() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) ||
+        TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value())
+        throw std::runtime_error("row operators: tracing (torch.jit.trace, make_fx, torch.export) is not provided");
+}
+
 // Gradients of gradients: where a graph of the backward pass is made, its results hang on an error node below everything that they
 // depend on, so that differentiating them is refused however it is reached.
 template <typename Grads>
 variable_list once(const variable_list& incoming, const variable_list& saved, Grads grads) {
+    untraced();
     variable_list out;
     {
         const at::NoGradGuard no_graph;
@@ -332,6 +343,7 @@ struct DropoutAddLayerNorm : torch::autograd::Function<DropoutAddLayerNorm> {
 
 // What the operators do not provide is an error.  (A dual tensor without a gradient would go past the nodes and lose its tangent.)
 void provided(std::initializer_list<const Tensor*> operands) {
+    untraced();
     if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
     for (const Tensor* t : operands)
         if (t->defined() && t->_fw_grad(0).defined()) throw std::runtime_error("row operators: forward-mode derivatives are not provided");

@@ -17,7 +17,8 @@ advance the tensor between steps (`rng[1] += calls_per_step`, also inside a capt
 forward pass keeps the two numbers it used, so the backward pass draws the same mask whatever happens to `rng` in between (activation
 checkpointing runs the forward pass again: advance `rng` after the backward pass there).
 
-Only `p = 0` works without an `rng`.  Gradients of gradients and forward-mode derivatives are not provided (an error).  The autograd nodes are csrc/row_autograd.cpp; here are
+Only `p = 0` works without an `rng`.  Gradients of gradients, forward-mode derivatives and tracing (torch.jit.trace, make_fx) are not
+provided: an error; torch.compile breaks its graph around a call.  The autograd nodes are csrc/row_autograd.cpp; here are
 the arguments and their checks."""
 import torch
 

@@ -216,3 +216,31 @@ def test_forward_mode_derivatives_are_refused(sim, name):
         with fwd._set_fwd_grad_enabled(False):
             assert torch.equal(op(dual), op(x))                    # nobody asks for one
         assert torch.equal(op(fwd.unpack_dual(dual).primal), op(x))
+
+
+@pytest.mark.parametrize('name', ['layer_norm', 'dropout', 'joined'])
+def test_tracing_is_refused(sim, name):
+    """A traced function would hold an allocation and no launch: torch.jit.trace, make_fx (before dispatch too) and torch.export are
+    errors, in the backward pass as well.  Modes that only watch the calls are not tracing."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    op, x = _ops(sim, row_ops.dropout_rng(0, 'cpu'))[name], make((4, 16), F32, 'cpu', 72)
+
+    class Module(torch.nn.Module):
+        def forward(self, t):
+            return op(t) + 1
+    with pytest.raises(RuntimeError, match='tracing'):
+        torch.jit.trace(lambda t: op(t) + 1, (x,), check_trace=False)
+    for kw in ({}, dict(pre_dispatch=True)):
+        with pytest.raises(RuntimeError, match='tracing'):
+            make_fx(lambda t: op(t) + 1, **kw)(x)
+    with pytest.raises(RuntimeError):                              # fake tensors have no memory, whoever notices first
+        make_fx(lambda t: op(t) + 1, tracing_mode='fake')(x)
+    with pytest.raises(Exception):
+        torch.export.export(Module(), (x,), strict=False)
+    leaf = x.clone().requires_grad_()
+    y = op(leaf)
+    with pytest.raises(RuntimeError, match='tracing'):
+        make_fx(lambda g: torch.autograd.grad(y, leaf, g, retain_graph=True)[0])(x)
+    with FlopCounterMode(display=False):
+        assert torch.equal(op(x), y.detach())
