@@ -72,8 +72,12 @@ Sizes sizes_of(const Tensor& x) {
     return {x.numel() / c, c};
 }
 
+// the tensor itself unless its memory holds its values negated (views such as the imaginary part of a conjugate)
+Tensor values_of(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // The tensor itself and the elements between its rows where they lie at one stride with their values side by side, else a copy.
-std::pair<Tensor, int64_t> rows_of(const Tensor& t) {
+std::pair<Tensor, int64_t> rows_of(const Tensor& given) {
+    const Tensor t = values_of(given);
     const int64_t last = t.dim() - 1, c = t.size(last);
     if (t.is_contiguous()) return {t, c};
     if (t.stride(last) == 1 || c == 1) {
@@ -178,6 +182,7 @@ const char* const kMeta = "m";
 // (an absent tensor is a nullopt to autograd and takes no place among a node's edges; inside, it is an undefined tensor)
 using Maybe = std::optional<Tensor>;
 Tensor or_none(const Maybe& t) { return t.has_value() ? *t : Tensor(); }
+Maybe resolved(const Maybe& t) { return t.has_value() ? Maybe(values_of(*t)) : t; }
 Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); }
 constexpr int64_t kNone = -1;
 int64_t type_or_none(const Tensor& t) { return t.defined() ? static_cast<int64_t>(t.scalar_type()) : kNone; }
@@ -350,7 +355,7 @@ void provided(std::initializer_list<const Tensor*> operands) {
 }
 
 // ---- what Python calls, with arguments that it has checked ------------------------------------------------------------------------
-Tensor dense(const Maybe& t) { return t.has_value() ? t->contiguous() : Tensor(); }
+Tensor dense(const Maybe& t) { return t.has_value() ? values_of(*t).contiguous() : Tensor(); }
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
 Tensor layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, double eps, int64_t entries, int64_t stream) {
@@ -362,21 +367,23 @@ Tensor layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, doubl
     return norm_forward(xr, ld, w, b, eps, to_of(entries, stream), Tensor());
 }
 
-Tensor dropout(const Tensor& x, const Maybe& residual, const Maybe& rng, const std::tuple<int64_t, int64_t, int64_t>& mask, int64_t call, int64_t entries,
+Tensor dropout(const Tensor& x, const Maybe& residual, const Maybe& rng_, const std::tuple<int64_t, int64_t, int64_t>& mask, int64_t call, int64_t entries,
                int64_t stream) {
     const OnDevice on(x);
     const Tensor r = or_none(residual);
+    const Maybe rng = resolved(rng_);
     provided({&x, &r});
     const auto [threshold, share, one_column] = mask;
     if (at::GradMode::is_enabled() && (wants(x) || wants(r))) return Dropout::apply(x, residual, rng, threshold, share, one_column, call, entries, stream);
     return drop(x, r, r.defined() ? r.scalar_type() : x.scalar_type(), {threshold, share, one_column}, numbers(or_none(rng)), call, nullptr, to_of(entries, stream));
 }
 
-std::pair<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const Tensor& residual, const Maybe& weight, const Maybe& bias, const Maybe& rng,
+std::pair<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const Tensor& residual, const Maybe& weight, const Maybe& bias, const Maybe& rng_,
                                                  const std::tuple<int64_t, int64_t, int64_t>& mask, int64_t call, double eps, bool inputs, int64_t entries,
                                                  int64_t stream) {
     const OnDevice on(x);
     const Tensor w = dense(weight), b = dense(bias);
+    const Maybe rng = resolved(rng_);
     provided({&x, &residual, &w, &b});
     const auto [threshold, share, one_column] = mask;
     variable_list out;

@@ -244,3 +244,44 @@ def test_tracing_is_refused(sim, name):
         make_fx(lambda g: torch.autograd.grad(y, leaf, g, retain_graph=True)[0])(x)
     with FlopCounterMode(display=False):
         assert torch.equal(op(x), y.detach())
+
+
+def test_compiled_functions_break_around_the_operators(sim):
+    x = make((4, 16), F32, 'cpu', 73)
+    for op in _ops(sim, row_ops.dropout_rng(0, 'cpu')).values():
+        assert torch.equal(torch.compile(lambda t: op(t * 2) + 1, backend='eager')(x), op(x * 2) + 1)
+
+
+# ---- tensors whose memory is not their values ----------------------------------------------------------------------------------
+def test_negative_views_are_read_as_their_values(on):  # noqa: F811
+    """A tensor with the negative bit (the imaginary part of a conjugate) as each operand, the mask's numbers and an incoming gradient."""
+    neg = lambda t: torch._neg_view(-t)                            # t's values over the memory of -t
+    x, r, w, b = make((3, 5, 16), F32, on.device, 74), make((3, 5, 16), F32, on.device, 75), make((16,), F32, on.device, 76), make((16,), F32, on.device, 77)
+    rng = row_ops.dropout_rng(6, on.device) + 3
+    assert neg(x).is_neg() and torch.equal(neg(x), x)
+    norm, drop, join = row_ops.layer_norm, row_ops.dropout, row_ops.dropout_add_layer_norm
+    want = norm(x, w, b, lib=on.lib)
+    for args in ((neg(x), w, b), (x, neg(w), b), (x, w, neg(b))):
+        assert torch.equal(norm(*args, lib=on.lib), want)
+        leaf = args[0].detach().requires_grad_()
+        assert torch.equal(norm(leaf, *args[1:], lib=on.lib), want)
+    assert torch.equal(drop(neg(x), 0.0, lib=on.lib), x)
+    want = drop(x, 0.5, rng, residual=r, lib=on.lib)
+    for a, g, s in ((neg(x), rng, r), (x, neg(rng), r), (x, rng, neg(r))):
+        assert torch.equal(drop(a, 0.5, g, residual=s, lib=on.lib), want)
+    want = join(x, r, w, b, 0.5, rng, lib=on.lib)
+    for a, s, p, q, g in ((neg(x), r, w, b, rng), (x, neg(r), w, b, rng), (x, r, neg(w), b, rng), (x, r, w, neg(b), rng), (x, r, w, b, neg(rng))):
+        assert all(torch.equal(u, v) for u, v in zip(join(a, s, p, q, 0.5, g, lib=on.lib), want))
+        got = join(a.detach().requires_grad_(), s, p, q, 0.5, g, lib=on.lib)
+        assert all(torch.equal(u, v) for u, v in zip(got, want))
+    one = make((7, 1), F32, on.device, 78)                         # (a column at any stride is read in place)
+    assert torch.equal(drop(neg(one), 0.0, lib=on.lib), one)
+
+    dy, dh = make((3, 5, 16), F32, on.device, 79), make((3, 5, 16), F32, on.device, 80)
+    leaves = [t.clone().requires_grad_() for t in (x, r, w)]
+    y = norm(leaves[0], leaves[2], lib=on.lib)
+    grads = lambda out, of, g: torch.autograd.grad(out, of, g, retain_graph=True)
+    for out, of, g, n in ((y, (leaves[0], leaves[2]), (dy,), (neg(dy),)), (drop(leaves[0], 0.5, rng, residual=leaves[1], lib=on.lib), leaves[:2], (dy,), (neg(dy),)),
+                          (join(*leaves, p=0.5, rng=rng, lib=on.lib), leaves, (dy, dh), (neg(dy), neg(dh))),
+                          (join(*leaves, p=0.5, rng=rng, lib=on.lib)[1], leaves[:2], (dh,), (neg(dh),))):
+        assert all(torch.equal(u, v) for u, v in zip(grads(out, of, g), grads(out, of, n)))
