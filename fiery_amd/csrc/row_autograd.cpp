@@ -59,9 +59,15 @@ struct OnDevice {
 
 int type_of(at::ScalarType t) { return t == at::kFloat ? FIERY_TYPE_F32 : t == at::kBFloat16 ? FIERY_TYPE_BF16 : FIERY_TYPE_F16; }
 int type_of(const Tensor& t) { return type_of(t.scalar_type()); }
-void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-float* floats(const Tensor& t, int64_t at = 0) { return t.defined() ? static_cast<float*>(t.data_ptr()) + at : nullptr; }
-int64_t* numbers(const Tensor& t) { return t.defined() ? static_cast<int64_t*>(t.data_ptr()) : nullptr; }
+// (null is an absent operand to the entry points: a tensor that has values and no memory, fake or zero, must not become one)
+void* ptr(const Tensor& t) {
+    if (!t.defined()) return nullptr;
+    void* p = t.data_ptr();
+    if (!p && t.numel()) throw std::runtime_error("row operators: a tensor without memory");
+    return p;
+}
+float* floats(const Tensor& t, int64_t at = 0) { return t.defined() ? static_cast<float*>(ptr(t)) + at : nullptr; }
+int64_t* numbers(const Tensor& t) { return static_cast<int64_t*>(ptr(t)); }
 Tensor dense_like(const Tensor& t, at::ScalarType type) { return at::empty(t.sizes(), t.options().dtype(type).requires_grad(false)); }
 
 struct Sizes {

@@ -285,3 +285,20 @@ def test_negative_views_are_read_as_their_values(on):  # noqa: F811
                           (join(*leaves, p=0.5, rng=rng, lib=on.lib), leaves, (dy, dh), (neg(dy), neg(dh))),
                           (join(*leaves, p=0.5, rng=rng, lib=on.lib)[1], leaves[:2], (dh,), (neg(dh),))):
         assert all(torch.equal(u, v) for u, v in zip(grads(out, of, g), grads(out, of, n)))
+
+
+def test_tensors_without_memory_are_refused(sim):
+    """Fake and zero tensors have no memory: an error, not an operand that is taken as absent (a residual that is not added, a weight of
+    ones) nor an address handed to a kernel."""
+    from torch._subclasses import FakeTensorMode
+    fake = FakeTensorMode()
+    x, w, rng = make((4, 16), F32, 'cpu', 81), make((16,), F32, 'cpu', 82), row_ops.dropout_rng(1, 'cpu')
+    norm, drop, join = row_ops.layer_norm, row_ops.dropout, row_ops.dropout_add_layer_norm
+    for empty in (lambda t: fake.from_tensor(t), lambda t: torch._efficientzerotensor(t.shape, dtype=t.dtype)):
+        for call in (lambda: norm(empty(x), lib=sim), lambda: norm(x, empty(w), lib=sim), lambda: norm(x, w, empty(w), lib=sim), lambda: drop(empty(x), 0.0, lib=sim),
+                     lambda: drop(x, 0.0, residual=empty(x), lib=sim), lambda: drop(x, 0.5, empty(rng), lib=sim), lambda: join(empty(x), x, lib=sim),
+                     lambda: join(x, empty(x), lib=sim), lambda: join(x, x, empty(w), w, lib=sim), lambda: join(x, x, w, empty(w), lib=sim),
+                     lambda: join(x, x, w, w, 0.5, empty(rng), lib=sim)):
+            with pytest.raises(RuntimeError):
+                call()
+    assert norm(torch.zeros(0, 16), w, lib=sim).shape == (0, 16)   # no rows need no memory
