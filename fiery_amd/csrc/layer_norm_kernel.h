@@ -311,6 +311,13 @@ __device__ __forceinline__ unsigned sum_again(const NormBwdArgs& a, const DropKe
     return bits;
 }
 
+// xhat of the columns that are none is (0 - mean) rstd, and 0 times it would be NaN in the row's sums where that overflows
+__device__ __forceinline__ void clear_far(float (&xhat)[kUnit], int count, float mean, float rstd) {
+    if (fabsf(mean * rstd) <= 3.4028234e38f) return;
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j) xhat[j] = j < count ? xhat[j] : 0.f;
+}
+
 // One unit of the backward pass's results from its dy (gg = dy gamma), xhat and the row's sums.
 template <typename T, typename S, bool JOIN, int RAGGED, bool SUM>
 __device__ __forceinline__ void store_grads(const NormBwdArgs& a, const DropKey& key, long long row, int unit, int count, const float (&gg)[kUnit],
@@ -400,16 +407,19 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_bwd(NormBwdArg
         }
         if (first + step < a.rows) fetch(first + step);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int j = 0; j < kUnit; ++j) xhat[i][j] = (xhat[i][j] - mean) * rstd;
+            clear_far(xhat[i], count[i], mean, rstd);                              // (past the row gg is 0)
 #pragma unroll
             for (int j = 0; j < kUnit; ++j) {
-                xhat[i][j] = (xhat[i][j] - mean) * rstd;                           // (past the row gg is 0)
                 dg[i][j] += gg[i][j] * xhat[i][j];
                 db[i][j] += gg[i][j];
                 gg[i][j] *= ga[i][j];
                 s[0] += gg[i][j];
                 s[1] += gg[i][j] * xhat[i][j];
             }
+        }
         row_sums<THREADS>(s, lanes, slots, turn);
         const float m1 = s[0] * a.inv_c, m2 = s[1] * a.inv_c;
 #pragma unroll
@@ -501,6 +511,7 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormBwdArgs a) {
                     xhat[j] = (xhat[j] - mean) * rstd;
                     gg[j] *= ga[j];
                 }
+                clear_far(xhat, count, mean, rstd);
                 if (walk == 0) {
 #pragma unroll
                     for (int j = 0; j < kUnit; ++j) {

@@ -302,3 +302,25 @@ def test_tensors_without_memory_are_refused(sim):
             with pytest.raises(RuntimeError):
                 call()
     assert norm(torch.zeros(0, 16), w, lib=sim).shape == (0, 16)   # no rows need no memory
+
+
+# ---- columns that are none -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('c', [9, 16, 24, 35, 72, 520, 1032, 2049, 2056, 8200, 8201])
+def test_gradients_of_far_rows_do_not_depend_on_the_width(on, c):  # noqa: F811
+    """|mean| rstd past the largest fp32 value: what the lanes behind a row's last column hold stays out of its sums, whether the width
+    fills its lanes (16) or not.  Rows of 1e33 with eps 1e-12 have xhat 0: dx = rstd (g - mean g), dweight takes nothing from them."""
+    skip_long(on, c > 2056)
+    x = make((4, c), F32, on.device, 83)
+    x[1], x[2] = 1e33, -1e33
+    leaf, w, dy = x.requires_grad_(), make((c,), F32, on.device, 84, 0.2, 1.0).requires_grad_(), make((4, c), F32, on.device, 85)
+    y = row_ops.layer_norm(leaf, w, None, 1e-12, lib=on.lib)
+    dx, dw = torch.autograd.grad(y, (leaf, w), dy)
+    g = dy[1:3].double().cpu() * w.detach().double().cpu()
+    want = (g - g.mean(-1, keepdim=True)) * 1e6
+    check_stored(dx[1:3], (want, ((depth(c) + 2) * U * g.abs().mean(-1, keepdim=True) + 4 * U * g.abs()) * 1e6 + 8 * U * want.abs()))
+    near = [0, 3]
+    check_stored(dw, grads_near(dy[near].double().cpu(), x[near].detach().double().cpu(), torch.zeros(2, c, dtype=torch.float64), w.detach(), 1e-12, None)[1])
+    if c <= 2049:
+        r = torch.zeros(4, c, device=on.device)
+        y, h = row_ops.dropout_add_layer_norm(leaf, r, w, eps=1e-12, lib=on.lib)
+        assert torch.equal(torch.autograd.grad(y, leaf, dy)[0], dx)
