@@ -4,24 +4,28 @@
 namespace fiery {
 namespace {
 
-// dgamma / dbeta = the sum of the workgroups' partial rows, 16 columns per workgroup: lane group r adds rows r, r + 64, ... in
+// dgamma / dbeta = the sum of the workgroups' partial rows, 16 columns at a time per workgroup: lane group r adds rows r, r + 64, ... in
 // double, then the 64 sums are added pairwise.  A fixed order: the same inputs give the same bits.
 __global__ __launch_bounds__(1024) void k_norm_finish(const float* __restrict__ partial, int blocks, int C, int width, void* dgamma, void* dbeta, int type) {
     __shared__ double lds[64][16];
-    const int col = threadIdx.x & 15, r = threadIdx.x >> 4, c = blockIdx.x * 16 + col;
+    const int col = threadIdx.x & 15, r = threadIdx.x >> 4;
     void* out = blockIdx.y ? dbeta : dgamma;
-    double s = 0.0;
-    if (c < C) {
-        const float* p = partial + static_cast<long long>(blockIdx.y) * width + c;
+    for (long long first = static_cast<long long>(blockIdx.x) * 16; first < C; first += static_cast<long long>(gridDim.x) * 16) {
+        const long long c = first + col;
+        double s = 0.0;
+        if (c < C) {
+            const float* p = partial + static_cast<long long>(blockIdx.y) * width + c;
 #pragma unroll 8
-        for (int b = r; b < blocks; b += 64) s += p[static_cast<long long>(b) * 2 * width];
+            for (int b = r; b < blocks; b += 64) s += p[static_cast<long long>(b) * 2 * width];
+        }
+        lds[r][col] = s;
+        for (int m = 32; m > 0; m >>= 1) {
+            __syncthreads();
+            if (r < m) lds[r][col] += lds[r + m][col];
+        }
+        if (r == 0 && c < C && out) store_typed(out, type, c, static_cast<float>(lds[0][col]));
+        __syncthreads();                                                   // (the next columns' sums go where these were read)
     }
-    lds[r][col] = s;
-    for (int m = 32; m > 0; m >>= 1) {
-        __syncthreads();
-        if (r < m) lds[r][col] += lds[r + m][col];
-    }
-    if (r == 0 && c < C && out) store_typed(out, type, c, static_cast<float>(lds[0][col]));
 }
 
 const char* norm_check(int64_t rows, int C, int x_type, int param_type, bool params) {
@@ -35,7 +39,8 @@ const char* norm_check(int64_t rows, int C, int x_type, int param_type, bool par
 
 void norm_finish(const NormBwdArgs& a, int blocks, hipStream_t stream) {
     const int width = (a.C + kUnit - 1) / kUnit * kUnit;
-    hipLaunchKernelGGL(k_norm_finish, dim3(ceil_div(a.C, 16), 2), dim3(1024), 0, stream, a.partial, blocks, a.C, width, a.dgamma, a.dbeta, a.param_type);
+    const int groups = ceil_div(a.C, 16), most = 8 * row_ops_cus();        // (a launch has fewer than 2^32 work-items: 2^26 columns would pass that)
+    hipLaunchKernelGGL(k_norm_finish, dim3(groups < most ? groups : most, 2), dim3(1024), 0, stream, a.partial, blocks, a.C, width, a.dgamma, a.dbeta, a.param_type);
 }
 
 }  // namespace fiery

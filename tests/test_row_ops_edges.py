@@ -324,3 +324,22 @@ def test_gradients_of_far_rows_do_not_depend_on_the_width(on, c):  # noqa: F811
         r = torch.zeros(4, c, device=on.device)
         y, h = row_ops.dropout_add_layer_norm(leaf, r, w, eps=1e-12, lib=on.lib)
         assert torch.equal(torch.autograd.grad(y, leaf, dy)[0], dx)
+
+
+# ---- sizes at the ends of the stated range -------------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_the_widest_parameters_gradient(hip):
+    """2^26 + 13 columns: sixteen of them to a workgroup of 1024 work-items are more than the 2^32 that a launch may have.  The first
+    and last columns are those of the definition over rows of two values (x = +-1 in turns: mean and spread known)."""
+    c = (1 << 26) + 13
+    sign = torch.ones(c, dtype=BF16, device='cuda')
+    sign[1::2] = -1.0
+    x = torch.stack((sign, -sign)).requires_grad_()
+    w = torch.ones(c, dtype=BF16, device='cuda', requires_grad=True)
+    b = torch.zeros(c, dtype=BF16, device='cuda', requires_grad=True)
+    y = row_ops.layer_norm(x, w, b, 0.0)
+    dy = torch.ones_like(y)
+    dy[1] = 2.0
+    dw, db = torch.autograd.grad(y, (w, b), dy)
+    # mean = +-1 / c (an odd count) and rstd = 1: xhat = x to 2^-26; dweight = 1 x - 2 x = -x, dbias = 1 + 2
+    assert torch.equal(dw, -sign) and torch.equal(db, torch.full_like(db, 3.0))
