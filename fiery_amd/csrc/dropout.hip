@@ -14,24 +14,13 @@
 namespace fiery {
 namespace {
 
-struct DropoutArgs {
-    const void* x;
-    const void* residual;
-    void* y;
-    long long x_ld, res_ld, y_ld;
-    int C;
-    unsigned total;                      // rows * units per row
-    FastDiv units;
-    DropArgs drop;
-};
-
 template <typename I, typename O, bool RES, int RAGGED>
 __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
     DropKey key = {0, 0, 0, 0};
     if (a.drop.threshold) key = drop_key(a.drop);
     drop_note(a.drop);
     for (unsigned long long q = static_cast<unsigned long long>(blockIdx.x) * 256 + threadIdx.x; q < a.total; q += static_cast<unsigned long long>(gridDim.x) * 256) {
-        const unsigned row = div_by(static_cast<unsigned>(q), a.units), unit = static_cast<unsigned>(q) - row * a.units.d;
+        const unsigned at = div_by(static_cast<unsigned>(q), a.units), row = a.first + at, unit = static_cast<unsigned>(q) - at * a.units.d;
         const long long c = static_cast<long long>(unit) * kUnit;
         const int count = RAGGED ? unit_count<RAGGED>(a.C, unit) : kUnit;
         float v[kUnit];
@@ -62,6 +51,32 @@ void dropout_launch(const DropoutArgs& a, hipStream_t stream) {
 }
 
 }  // namespace
+
+// (as many launches as keep the flat index below 2^31: a launch's rows start at `first`, which the mask counts too)
+void dropout_rows(DropoutArgs a, int64_t rows, int x_type, int y_type, hipStream_t stream) {
+    const int64_t units = (static_cast<int64_t>(a.C) + kUnit - 1) / kUnit, most = ((1ll << 31) - 1) / units;
+    a.units = fast_div(static_cast<unsigned>(units));
+    for (int64_t first = 0; first < rows; first += most) {
+        a.first = static_cast<unsigned>(first);
+        a.total = static_cast<unsigned>((rows - first < most ? rows - first : most) * units);
+        if (first > 0) a.drop.rng_used = nullptr;
+        if (x_type == FIERY_TYPE_F32 && y_type == FIERY_TYPE_F32)
+            dropout_launch<F32, F32>(a, stream);
+        else if (x_type == FIERY_TYPE_BF16 && y_type == FIERY_TYPE_BF16)
+            dropout_launch<BF16, BF16>(a, stream);
+        else if (x_type == FIERY_TYPE_F16 && y_type == FIERY_TYPE_F16)
+            dropout_launch<F16, F16>(a, stream);
+        else if (x_type == FIERY_TYPE_BF16)
+            dropout_launch<BF16, F32>(a, stream);
+        else if (x_type == FIERY_TYPE_F16)
+            dropout_launch<F16, F32>(a, stream);
+        else if (y_type == FIERY_TYPE_BF16)
+            dropout_launch<F32, BF16>(a, stream);
+        else
+            dropout_launch<F32, F16>(a, stream);
+    }
+}
+
 }  // namespace fiery
 
 using namespace fiery;
@@ -86,22 +101,6 @@ extern "C" int fiery_dropout(const void* x, int64_t x_ld, int x_type, const void
     a.res_ld = res_ld;
     a.y_ld = y_ld;
     a.C = C;
-    a.total = static_cast<unsigned>(rows * units);
-    a.units = fast_div(static_cast<unsigned>(units));
-    hipStream_t hs = as_stream(stream);
-    if (x_type == FIERY_TYPE_F32 && y_type == FIERY_TYPE_F32)
-        dropout_launch<F32, F32>(a, hs);
-    else if (x_type == FIERY_TYPE_BF16 && y_type == FIERY_TYPE_BF16)
-        dropout_launch<BF16, BF16>(a, hs);
-    else if (x_type == FIERY_TYPE_F16 && y_type == FIERY_TYPE_F16)
-        dropout_launch<F16, F16>(a, hs);
-    else if (x_type == FIERY_TYPE_BF16)
-        dropout_launch<BF16, F32>(a, hs);
-    else if (x_type == FIERY_TYPE_F16)
-        dropout_launch<F16, F32>(a, hs);
-    else if (y_type == FIERY_TYPE_BF16)
-        dropout_launch<F32, BF16>(a, hs);
-    else
-        dropout_launch<F32, F16>(a, hs);
+    dropout_rows(a, rows, x_type, y_type, as_stream(stream));
     return check_launch("dropout");
 }

@@ -59,13 +59,26 @@ int join_bwd(const void* dy, int64_t dy_ld, const void* dh, int64_t dh_ld, const
              int64_t rows, int C, const void* gamma, int param_type, const float* mean, const float* rstd, int threshold, const int64_t* rng_used,
              int64_t rows_per_mask, int one_column, void* dx, int64_t dx_ld, void* dresidual, int64_t dres_ld, void* dgamma, void* dbeta, float* workspace,
              int64_t workspace_floats, fiery_stream_t stream) {
-    FIERY_REQUIRE(dy && h && mean && rstd && (dx || dresidual || dgamma || dbeta), "dropout_add_layer_norm_bwd: null pointer");
+    const bool h_alone = !dy;                                              // only h went on: dx is the dropout of dh, dresidual is dh itself
+    FIERY_REQUIRE(h_alone ? dh && dx && !dresidual && !dgamma && !dbeta : h && mean && rstd && (dx || dresidual || dgamma || dbeta),
+                  "dropout_add_layer_norm_bwd: null pointer");
     NormBwdArgs a = {};
     const char* bad = join_check(rows, C, x_type, stream_type, param_type, gamma || dgamma || dbeta);
     if (!bad) bad = drop_args(a.drop, rng_used, nullptr, 0, threshold, rows_per_mask, one_column);
     FIERY_REQUIRE(!bad, "dropout_add_layer_norm_bwd: %s", bad);
     FIERY_REQUIRE(dy_ld >= 0 && h_ld >= 0 && x_ld >= 0 && (!dh || dh_ld >= 0) && (!dx || dx_ld >= C) && (!dresidual || dres_ld >= C),
                   "dropout_add_layer_norm_bwd: bad row stride");
+    if (h_alone) {
+        DropoutArgs d = {};
+        d.x = dh;
+        d.y = dx;
+        d.x_ld = dh_ld;
+        d.y_ld = dx_ld;
+        d.C = C;
+        d.drop = a.drop;
+        dropout_rows(d, rows, stream_type, x_type, as_stream(stream));
+        return check_launch("dropout_add_layer_norm_bwd");
+    }
     if ((dgamma || dbeta) && norm_bwd_workspace_floats(rows, C) > 0) {
         FIERY_REQUIRE(workspace, "dropout_add_layer_norm_bwd: null workspace");
         if (workspace_floats < norm_bwd_workspace_floats(rows, C)) return fail(FIERY_ENOMEM, "dropout_add_layer_norm_bwd: workspace too small");

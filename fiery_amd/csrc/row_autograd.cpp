@@ -322,8 +322,14 @@ struct DropoutAddLayerNorm : torch::autograd::Function<DropoutAddLayerNorm> {
             const bool want_x = ctx->needs_input_grad(0), want_r = ctx->needs_input_grad(1);
             Tensor dx, dr;
             if (!dy.defined()) {                                        // only h went on: there is no norm to differentiate
-                s.rows = 0;
-                if (want_x && dh.defined()) dx = drop(dh, Tensor(), x_type, m, used, 0, nullptr, to);
+                const int64_t rows = std::exchange(s.rows, 0);
+                if (want_x && dh.defined()) {
+                    dx = dense_like(h, x_type);
+                    const auto [hg, dh_ld] = rows_of(dh);
+                    if (rows) check(to, to.lib->join_bwd(nullptr, 0, ptr(hg), dh_ld, nullptr, 0, type_of(x_type), type_of(h), rows, static_cast<int>(s.c), nullptr, 0,
+                                                         nullptr, nullptr, static_cast<int>(m.threshold), used, m.share, static_cast<int>(m.one_column), ptr(dx),
+                                                         s.c, nullptr, 0, nullptr, nullptr, nullptr, 0, to.stream));
+                }
                 if (want_r) dr = dh;
             } else {
                 if (want_x) dx = dense_like(h, x_type);

@@ -325,6 +325,18 @@ inline const char* drop_args(DropArgs& d, const void* rng, void* rng_used, int64
     return nullptr;
 }
 
+struct DropoutArgs {
+    const void* x;
+    const void* residual;
+    void* y;
+    long long x_ld, res_ld, y_ld;
+    int C;
+    unsigned first, total;               // of a launch: its first row, its rows * units per row
+    FastDiv units;
+    DropArgs drop;
+};
+void dropout_rows(DropoutArgs a, int64_t rows, int x_type, int y_type, hipStream_t stream);          // dropout.hip
+
 inline bool row_type(int t) { return t == FIERY_TYPE_F32 || t == FIERY_TYPE_BF16 || t == FIERY_TYPE_F16; }
 
 }  // namespace fiery

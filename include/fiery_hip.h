@@ -587,7 +587,8 @@ int fiery_dropout(const void* x, int64_t x_ld, int x_type, const void* residual,
 /* h = residual + dropout(x), y = layer norm(h): one pass.  residual, h and their gradients are of stream_type (the rows' type or
  * fp32); y comes from h before it is rounded to that type, mean and rstd are those of the h that is stored, which the backward pass
  * reads: its gradients are the norm's at that h.  Backward: dh = the gradient of h itself or NULL;
- * dresidual = dh + d(layer norm), dx = dropout of it; every output may be NULL, not all.  Mask, statistics, workspace: as above. */
+ * dresidual = dh + d(layer norm), dx = dropout of it; every output may be NULL, not all.  dy NULL: h alone went on and dx, the dropout of
+ * dh, is the only output (dresidual is dh; h, mean and rstd may be NULL).  Mask, statistics, workspace: as above. */
 int fiery_dropout_add_layer_norm_fwd(const void* x, int64_t x_ld, int x_type, const void* residual, int64_t res_ld, int stream_type, int64_t rows,
                                      int C, const void* gamma, const void* beta, int param_type, float eps, int threshold, const int64_t* rng,
                                      int64_t call, int64_t rows_per_mask, int one_column, int64_t* rng_used, void* y, int64_t y_ld, void* h,

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from fiery_amd import native, row_ops
-from tests.test_row_ops import BF16, F16, F32, U, Backend, check_stored, depth, kept, make, norm64, on, skip_long, xhat_error  # noqa: F401
+from tests.test_row_ops import BF16, F16, F32, U, check_stored, depth, kept, make, norm64, on, philox, skip_long, xhat_error  # noqa: F401
 
 
 # ---- gradients of the joined operator at the h before its rounding -----------------------------------------------------------
@@ -343,3 +343,41 @@ def test_the_widest_parameters_gradient(hip):
     dw, db = torch.autograd.grad(y, (w, b), dy)
     # mean = +-1 / c (an odd count) and rstd = 1: xhat = x to 2^-26; dweight = 1 x - 2 x = -x, dbias = 1 + 2
     assert torch.equal(dw, -sign) and torch.equal(db, torch.full_like(db, 3.0))
+
+
+@pytest.mark.parametrize('per', ['element', 'channel', 'sample'])
+@pytest.mark.parametrize('dtype,stream', [(F32, F32), (BF16, BF16), (F16, F16), (BF16, F32), (F16, F32)], ids=str)
+def test_the_gradient_of_h_alone_at_the_entry_point(on, per, dtype, stream):  # noqa: F811
+    """dy null: only h went on; dx is the dropout of dh, the mask that of the forward pass."""
+    shape, lib = (3, 4, 21), native.get() if on.device == 'cuda' else on.lib
+    rng, dh = row_ops.dropout_rng(5, on.device), make(shape, stream, on.device, 86)
+    dx = torch.empty(shape, dtype=dtype, device=on.device)
+    t, s, share = native.ROW_TYPES[dtype], native.ROW_TYPES[stream], 1 if per == 'element' else 4
+    at = torch.cuda.current_stream().cuda_stream if on.device == 'cuda' else None
+    call = lambda dy=None, dh=dh.data_ptr(), dres=None, dg=None: lib.check(lib.dll.fiery_dropout_add_layer_norm_bwd(
+        dy, 21, dh, 21, None, 0, t, s, 12, 21, None, 0, None, None, 19661, rng.data_ptr(), share, per == 'sample', dx.data_ptr(), 21, dres, 21, dg, None, None, 0, at))
+    call()
+    want = dh.double().cpu() * kept(shape, 19661 / 65536, 5, 0, per)
+    check_stored(dx, (want, 2 * U * want.abs()))
+    if on.device == 'cpu':
+        p = torch.zeros(300).data_ptr()
+        for kw in (dict(dh=None), dict(dy=p), dict(dres=p), dict(dg=p)):
+            with pytest.raises(native.NativeError):
+                call(**kw)
+
+
+@pytest.mark.gpu
+def test_the_gradient_of_h_alone_past_two_billion_units(hip):
+    """2^30 + 5 rows of nine columns are 2^31 + 10 units of eight: the forward pass takes them, and so does the gradient of h alone."""
+    rows, c = (1 << 30) + 5, 9
+    x = make((1, c), BF16, 'cuda', 87).expand(rows, c).requires_grad_()
+    dh = make((1, c), BF16, 'cuda', 88).expand(rows, c)
+    rng = row_ops.dropout_rng(13, 'cuda')
+    y, h = row_ops.dropout_add_layer_norm(x, x.detach(), p=0.5, rng=rng)
+    del y
+    dx, = torch.autograd.grad(h, x, dh)
+    for first in (0, (1 << 30) - 4, rows - 7):
+        words = [[v >> 16 * k & 0xffff for unit in range(2) for v in philox([unit, first + i, 0, 0], [13, 0]) for k in range(2)][:c] for i in range(7)]
+        keep = torch.tensor(words, device='cuda') >= 32768
+        assert torch.equal(dx[first:first + 7], torch.where(keep, dh[:7] * 2, torch.zeros_like(dh[:7]))), first
+    assert torch.equal(h[-7:], x.detach()[:7] + torch.where(keep, x.detach()[:7] * 2, torch.zeros_like(dh[:7])))
