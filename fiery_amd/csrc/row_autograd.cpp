@@ -409,6 +409,7 @@ std::pair<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const Tensor& 
 }  // namespace
 
 PYBIND11_MODULE(_row_autograd, m) {
+    m.attr("abi_version") = FIERY_ABI_VERSION;
     m.def("rows_of", &rows_of);
     m.def("layer_norm", &layer_norm);
     m.def("dropout", &dropout);

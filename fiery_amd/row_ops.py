@@ -36,6 +36,9 @@ def _autograd():
             from . import _row_autograd
         except ImportError as e:
             raise native.NativeError(f'fiery_amd/_row_autograd.so does not load ({e}): build it first (`python -m fiery_amd.build`)') from e
+        got = getattr(_row_autograd, 'abi_version', None)
+        if got != native.ABI_VERSION:
+            raise native.NativeError(f'fiery_amd/_row_autograd.so: ABI version {got}, bindings expect {native.ABI_VERSION}; rebuild')
         _nodes = _row_autograd
     return _nodes
 

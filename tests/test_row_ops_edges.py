@@ -381,3 +381,19 @@ def test_the_gradient_of_h_alone_past_two_billion_units(hip):
         keep = torch.tensor(words, device='cuda') >= 32768
         assert torch.equal(dx[first:first + 7], torch.where(keep, dh[:7] * 2, torch.zeros_like(dh[:7]))), first
     assert torch.equal(h[-7:], x.detach()[:7] + torch.where(keep, x.detach()[:7] * 2, torch.zeros_like(dh[:7])))
+
+
+# ---- the two libraries ---------------------------------------------------------------------------------------------------------
+def test_nodes_built_against_another_header_are_refused(sim, monkeypatch):
+    """The nodes call the library by address with their own header's signatures: a stale build is an error, as a stale library is."""
+    import types
+    old = types.SimpleNamespace(abi_version=native.ABI_VERSION - 1, rows_of=None)
+    monkeypatch.setattr(row_ops, '_nodes', None)
+    monkeypatch.setitem(sys.modules, 'fiery_amd._row_autograd', old)
+    monkeypatch.setattr('fiery_amd._row_autograd', old, raising=False)
+    with pytest.raises(native.NativeError, match='ABI'):
+        row_ops.layer_norm(torch.ones(2, 8), lib=sim)
+    monkeypatch.setitem(sys.modules, 'fiery_amd._row_autograd', types.SimpleNamespace(rows_of=None))
+    monkeypatch.delattr('fiery_amd._row_autograd', raising=False)
+    with pytest.raises(native.NativeError, match='ABI'):           # from before the number was there
+        row_ops.layer_norm(torch.ones(2, 8), lib=sim)
