@@ -227,6 +227,7 @@ EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 ROW_ENTRIES = ('fiery_last_error', 'fiery_layer_norm_fwd', 'fiery_layer_norm_bwd_workspace_floats', 'fiery_layer_norm_bwd', 'fiery_dropout',
                'fiery_dropout_add_layer_norm_fwd', 'fiery_dropout_add_layer_norm_bwd', 'fiery_dropout_add_layer_norm_fwd_unrounded',
                'fiery_dropout_add_layer_norm_bwd_unrounded')
+_ROW_TABLES = []                 # every table of their addresses: autograd graphs hold them by address, past the `Lib` that made them
 
 
 def require_usable_gpu_process(what):
@@ -322,6 +323,7 @@ class Lib:
             fn = getattr(self.dll, name)          # AttributeError here = symbol missing from the build
             fn.restype, fn.argtypes = restype, argtypes
         self._row_entries = (C.c_void_p * len(ROW_ENTRIES))(*[C.cast(getattr(self.dll, name), C.c_void_p).value for name in ROW_ENTRIES])
+        _ROW_TABLES.append(self._row_entries)
         self.row_entries = C.addressof(self._row_entries)
         self.launches_on_gpu = hasattr(self.dll, 'hipLaunchKernel')       # (False: the CPU simulator's build of the sources)
         self.dll = _EntryPoints(self.dll)

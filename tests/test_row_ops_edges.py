@@ -397,3 +397,19 @@ def test_nodes_built_against_another_header_are_refused(sim, monkeypatch):
     monkeypatch.delattr('fiery_amd._row_autograd', raising=False)
     with pytest.raises(native.NativeError, match='ABI'):           # from before the number was there
         row_ops.layer_norm(torch.ones(2, 8), lib=sim)
+
+
+def test_a_graph_outlives_the_library_object_it_was_made_with(sim):
+    """Nodes keep the address of the library's table of entry points: it stays, whatever becomes of the object that made it."""
+    import gc
+    import weakref
+    lib = native.Lib(sim.path)
+    x = make((4, 24), F32, 'cpu', 90).requires_grad_()
+    dy = make((4, 24), F32, 'cpu', 91)
+    y = row_ops.layer_norm(x, lib=lib)
+    want, = torch.autograd.grad(y, x, dy, retain_graph=True)
+    table, gone = weakref.ref(lib._row_entries), weakref.ref(lib)
+    del lib
+    gc.collect()
+    assert gone() is None and table() is not None
+    assert torch.equal(torch.autograd.grad(y, x, dy)[0], want)
