@@ -276,8 +276,9 @@ def warp_flags_of_this_host(h, w):
     return _WARP_FLAGS[key]
 
 
-# `CALL_SINK = []`: every launching entry point of the library that is called through `Lib` (the row operators are not) is bracketed by HIP events on the current stream and filed as
-# (entry point, start, end) - bench.py's per-kernel table of the pass from images (None: the calls go straight through)
+# `CALL_SINK = []`: every launching entry point of the library that is called through `Lib` or by the row operators is bracketed by HIP
+# events on the current stream and filed as (entry point, start, end) - bench.py's per-kernel table of the pass from images (None: the
+# calls go straight through; a graph of the row operators goes the way of its forward pass)
 CALL_SINK = None
 _HOST_ONLY = ('version', 'last_error', 'workspace_', 'occupied_offset', 'packed_floats', '_plan', '_used')
 
@@ -324,12 +325,28 @@ class Lib:
             fn.restype, fn.argtypes = restype, argtypes
         self._row_entries = (C.c_void_p * len(ROW_ENTRIES))(*[C.cast(getattr(self.dll, name), C.c_void_p).value for name in ROW_ENTRIES])
         _ROW_TABLES.append(self._row_entries)
-        self.row_entries = C.addressof(self._row_entries)
+        self._timed_row_entries = None
         self.launches_on_gpu = hasattr(self.dll, 'hipLaunchKernel')       # (False: the CPU simulator's build of the sources)
         self.dll = _EntryPoints(self.dll)
         got = self.dll.fiery_abi_version()
         if got != ABI_VERSION:
             raise NativeError(f'{path}: ABI version {got}, bindings expect {ABI_VERSION}; rebuild')
+
+    @property
+    def row_entries(self):
+        """The address of the table that csrc/row_autograd.cpp calls through."""
+        if CALL_SINK is None:
+            return C.addressof(self._row_entries)
+        if self._timed_row_entries is None:          # calls back into `_EntryPoints`, which brackets and files them
+            made, table = [], (C.c_void_p * len(ROW_ENTRIES))(*self._row_entries)
+            for i, name in enumerate(ROW_ENTRIES):
+                if not any(t in name for t in _HOST_ONLY):
+                    restype, argtypes = _SIGNATURES[name]
+                    made.append(C.CFUNCTYPE(restype, *argtypes)(getattr(self.dll, name)))
+                    table[i] = C.cast(made[-1], C.c_void_p).value
+            _ROW_TABLES.append((table, made))
+            self._timed_row_entries = table
+        return C.addressof(self._timed_row_entries)
 
     def check(self, rc):
         if rc != 0:

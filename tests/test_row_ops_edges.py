@@ -413,3 +413,40 @@ def test_a_graph_outlives_the_library_object_it_was_made_with(sim):
     gc.collect()
     assert gone() is None and table() is not None
     assert torch.equal(torch.autograd.grad(y, x, dy)[0], want)
+
+
+def _timed_step(lib, device):
+    x, r = make((4, 24), F32, device, 92).requires_grad_(), make((4, 24), F32, device, 93).requires_grad_()
+    w, rng = make((24,), F32, device, 94, 0.2, 1.0).requires_grad_(), row_ops.dropout_rng(3, device)
+    y, h = row_ops.dropout_add_layer_norm(row_ops.layer_norm(x, w, lib=lib), row_ops.dropout(r, 0.3, rng, lib=lib), w, p=0.2, rng=rng, call=1, lib=lib)
+    return [y, h, *torch.autograd.grad((y, h), (x, r, w), (make((4, 24), F32, device, 95), make((4, 24), F32, device, 96)))]
+
+
+def test_the_call_table_sees_the_row_operators(on, monkeypatch):  # noqa: F811
+    """native.CALL_SINK: forward and backward launches of the row operators are filed as the library's others are, and compute what they do
+    without it; a graph that was made with the table open works when it is closed again."""
+    if on.device == 'cpu':                                         # (no events there: stand-ins)
+        class Event:
+            def __init__(self, enable_timing):
+                self.recorded = 0
+
+            def record(self):
+                self.recorded += 1
+        monkeypatch.setattr(torch.cuda, 'is_available', lambda: True)
+        monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: False)
+        monkeypatch.setattr(torch.cuda, 'Event', Event)
+    want = _timed_step(on.lib, on.device)
+    monkeypatch.setattr(native, 'CALL_SINK', [])
+    got = _timed_step(on.lib, on.device)
+    names = [name for name, _, _ in native.CALL_SINK]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert sorted(names) == sorted(['fiery_layer_norm_fwd', 'fiery_dropout', 'fiery_dropout_add_layer_norm_fwd', 'fiery_dropout_add_layer_norm_bwd',
+                                    'fiery_layer_norm_bwd', 'fiery_dropout'])
+    if on.device == 'cuda':
+        torch.cuda.synchronize()
+        assert all(start.elapsed_time(end) >= 0.0 for _, start, end in native.CALL_SINK)
+    leaf = make((4, 24), F32, on.device, 97).requires_grad_()
+    y = row_ops.layer_norm(leaf, lib=on.lib)
+    monkeypatch.setattr(native, 'CALL_SINK', None)
+    dx, = torch.autograd.grad(y, leaf, torch.ones_like(y))
+    assert torch.equal(dx, torch.autograd.grad(row_ops.layer_norm(leaf, lib=on.lib), leaf, torch.ones_like(y))[0])
