@@ -15,7 +15,7 @@ p is drawn as round(65536 p) / 65536 and what is kept is scaled by the inverse o
 int64 [seed, call] (`dropout_rng`); `call=` is added to its second number.  Give every dropout of a step its own number and
 advance the tensor between steps (`rng[1] += calls_per_step`, also inside a captured graph: replays then draw new masks).  The
 forward pass keeps the two numbers it used, so the backward pass draws the same mask whatever happens to `rng` in between (activation
-checkpointing runs the forward pass again: advance `rng` after the backward pass there).
+checkpointing runs the forward pass again: advance `rng` after the backward pass there; the training graph sees to it by itself).
 
 Only `p = 0` works without an `rng`.  Gradients of gradients, forward-mode derivatives and tracing (torch.jit.trace, make_fx) are not
 provided: an error; torch.compile breaks its graph around a call.  The autograd nodes are csrc/row_autograd.cpp; here are

@@ -123,6 +123,10 @@ if DROP_CONNECT not in ('torch', 'counter'):
     raise ValueError(f"FIERY_TRAIN_DROP_CONNECT is 'torch' or 'counter', got {DROP_CONNECT!r}")
 
 
+def _capturing(x):
+    return x.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 def _train_forms():
     """The optional weight images a training convolution packs (per call: the weights change every step)."""
     if not TRAIN_WINOGRAD or CONV_PRECISION != native.PRECISION_F32:
@@ -670,7 +674,12 @@ class TrainGraph:
         """skip + dropout(x) of (N, C, H, W) tensors in one launch (`row_ops.dropout`): per 'channel' (`nn.Dropout2d`) or 'sample'
         (drop-connect).  The masks are numbered by `model.dropout_rng` ([seed, call] on the device, made from torch's global seed
         at its first use; set it to choose them) and the dropout's place in the pass; the pass advances the tensor when it ends,
-        so replays of a captured step draw new masks."""
+        so replays of a captured step draw new masks.
+
+        Under activation checkpointing (`torch.utils.checkpoint(..., use_reentrant=False)`; any hooks on saved tensors count as such) the
+        pass runs again inside the backward pass, when the tensor has moved on.  The number is then drawn from torch's CPU generator,
+        whose state checkpoint restores, and the tensor gives the seed alone.  A reentrant checkpoint's first pass cannot be told from
+        any other: its second one is refused, and so is a captured one (every replay would draw the same masks)."""
         if not self._hip_ops:                         # tests: a substituted convolution, any type or device
             shape = (x.shape[0], x.shape[1], 1, 1) if per == 'channel' else (x.shape[0], 1, 1, 1)
             return skip + x * F.dropout(x.new_ones(shape), p)
@@ -679,7 +688,19 @@ class TrainGraph:
         if rng is None or rng.device != x.device:
             rng = row_ops.dropout_rng(int(torch.randint(1 << 62, (1,))), x.device) if rng is None else rng.to(x.device)
             owner.__dict__['dropout_rng'] = rng
-        y = row_ops.dropout(x.float().permute(0, 2, 3, 1), p, rng, call=self._dropouts, per=per, residual=skip.float().permute(0, 2, 3, 1), lib=self.lib)
+        call, again = self._dropouts, torch._C._autograd._top_saved_tensors_default_hooks(False) is not None
+        if again:
+            if _capturing(x):
+                raise RuntimeError('dropout under saved-tensor hooks (activation checkpointing) cannot be captured into a graph')
+            call = int(torch.randint(1 << 62, (1,)))
+            rng = rng.clone()
+            rng[1:].zero_()
+        elif torch._C._current_graph_task_id() != -1:
+            raise RuntimeError('dropout inside a backward pass: a reentrant checkpoint runs its forward pass again there and would draw '
+                               'other masks; use torch.utils.checkpoint.checkpoint(..., use_reentrant=False)')
+        y = row_ops.dropout(x.float().permute(0, 2, 3, 1), p, rng, call=call, per=per, residual=skip.float().permute(0, 2, 3, 1), lib=self.lib)
+        if again:
+            return y.permute(0, 3, 1, 2)
         self._dropouts += 1
         if self._counters is None:                    # a block on its own: no pass to number it in
             self._advance_dropout()
