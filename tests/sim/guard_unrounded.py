@@ -36,10 +36,10 @@ def main():
             stats, used = guarded(torch.rand(2 * rows) + 0.5, where), guarded(torch.zeros(2, dtype=torch.int64), where)
             mean, rstd = stats.data_ptr(), stats.data_ptr() + 4 * rows
             ws = given((n,), torch.float32) if n else None
-            for threshold, share, one in ((20000, 1, 0), (20000, 2, 1), (0, 1, 0)):
+            for threshold, share, one in ((20000, 1, 0), (20000, 2, 1), (0, 1, 0))[:1 if c > 8000 else 3]:
                 lib.check(lib.dll.fiery_dropout_add_layer_norm_fwd_unrounded(x(), c, t, x(), c, t, rows, c, par(), par(), t, 1e-5, threshold, rng.data_ptr(), 1, share,
                                                                              one, used.data_ptr(), x(), c, x(), c, mean, rstd, None))
-                for dh in (None, x()):
+                for dh in (None, x())[1 if c > 8000 else 0:]:
                     lib.check(lib.dll.fiery_dropout_add_layer_norm_bwd_unrounded(x(), c, dh, c, x(), c, x(), c, t, rows, c, par(), t, mean, rstd, threshold,
                                                                                  used.data_ptr(), share, one, x(), c, x(), c, par(), par(), ws, n, None))
             done += 1
