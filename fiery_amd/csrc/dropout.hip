@@ -24,10 +24,10 @@ __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
         const long long c = static_cast<long long>(unit) * kUnit;
         const int count = RAGGED ? unit_count<RAGGED>(a.C, unit) : kUnit;
         float v[kUnit];
-        load_unit<I, RAGGED>(static_cast<const typename I::store*>(a.x) + row * a.x_ld + c, count, a.C, v);
+        load_unit<I, RAGGED>(static_cast<const typename I::store*>(a.x) + row * a.x_ld + c, count, v);
         if constexpr (RES) {
             float r[kUnit];
-            load_unit<O, RAGGED>(static_cast<const typename O::store*>(a.residual) + row * a.res_ld + c, count, a.C, r);
+            load_unit<O, RAGGED>(static_cast<const typename O::store*>(a.residual) + row * a.res_ld + c, count, r);
             drop_unit(a.drop, key, row, unit, v);
 #pragma unroll
             for (int j = 0; j < kUnit; ++j) v[j] += r[j];

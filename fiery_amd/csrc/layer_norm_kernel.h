@@ -115,14 +115,14 @@ __device__ __forceinline__ float rstd_of(float x) {
 template <typename T, typename S, bool JOIN, int RAGGED>
 __device__ __forceinline__ void load_h(const NormFwdArgs& a, const DropKey& key, long long row, bool live, int unit, int count, bool write, float (&v)[kUnit]) {
     const long long c = static_cast<long long>(unit) * kUnit;
-    const Raw<T> x = load_raw<T, RAGGED>(static_cast<const typename T::store*>(a.x) + row * a.x_ld + c, live, count, a.C);
+    const Raw<T> x = load_raw<T, RAGGED>(static_cast<const typename T::store*>(a.x) + row * a.x_ld + c, live, count);
     if constexpr (!JOIN) {
-        unpack<T, RAGGED>(x, count, a.C, v);
+        unpack<T, RAGGED>(x, count, v);
     } else {
-        const Raw<S> residual = load_raw<S, RAGGED>(static_cast<const typename S::store*>(a.residual) + row * a.res_ld + c, live, count, a.C);
+        const Raw<S> residual = load_raw<S, RAGGED>(static_cast<const typename S::store*>(a.residual) + row * a.res_ld + c, live, count);
         float r[kUnit];
-        unpack<T, RAGGED>(x, count, a.C, v);
-        unpack<S, RAGGED>(residual, count, a.C, r);
+        unpack<T, RAGGED>(x, count, v);
+        unpack<S, RAGGED>(residual, count, r);
         drop_unit(a.drop, key, static_cast<unsigned>(row), static_cast<unsigned>(unit), v);
 #pragma unroll
         for (int j = 0; j < kUnit; ++j) v[j] += r[j];
@@ -190,8 +190,8 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_fwd(NormFwdArg
     for (int i = 0; i < NV; ++i) {
         const int unit = i * lanes + sub;
         count[i] = unit_count<RAGGED>(a.C, unit);
-        load_typed<RAGGED>(a.gamma, a.param_type, static_cast<long long>(unit) * kUnit, count[i], a.C, 1.f, ga[i]);
-        load_typed<RAGGED>(a.beta, a.param_type, static_cast<long long>(unit) * kUnit, count[i], a.C, 0.f, be[i]);
+        load_typed<RAGGED>(a.gamma, a.param_type, static_cast<long long>(unit) * kUnit, count[i], 1.f, ga[i]);
+        load_typed<RAGGED>(a.beta, a.param_type, static_cast<long long>(unit) * kUnit, count[i], 0.f, be[i]);
     }
     // (every lane of a wavefront walks the loop as often as its neighbours: the exchanges need all of them)
     for (long long first = static_cast<long long>(blockIdx.x) * per_block; first < a.rows; first += static_cast<long long>(gridDim.x) * per_block) {
@@ -287,8 +287,8 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_long(NormFwdArgs a) {
             const int count = unit_count<2>(a.C, u);
             load_h<T, S, JOIN, 2>(a, key, row, true, u, count, false, v);
             float ga[kUnit], be[kUnit];
-            load_typed<2>(a.gamma, a.param_type, static_cast<long long>(u) * kUnit, count, a.C, 1.f, ga);
-            load_typed<2>(a.beta, a.param_type, static_cast<long long>(u) * kUnit, count, a.C, 0.f, be);
+            load_typed<2>(a.gamma, a.param_type, static_cast<long long>(u) * kUnit, count, 1.f, ga);
+            load_typed<2>(a.beta, a.param_type, static_cast<long long>(u) * kUnit, count, 0.f, be);
 #pragma unroll
             for (int j = 0; j < kUnit; ++j) v[j] = (v[j] - mean) * rstd * ga[j] + be[j];
             store_unit<T, 2>(static_cast<typename T::store*>(a.y) + row * a.y_ld + static_cast<long long>(u) * kUnit, count, v);
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_long(NormFwdArgs a) {
 template <typename T, int RAGGED>
 __device__ __forceinline__ unsigned sum_again(const NormBwdArgs& a, const DropKey& key, long long row, int unit, int count, const Raw<T>& x, float (&v)[kUnit]) {
     float d[kUnit];
-    unpack<T, RAGGED>(x, count, a.C, d);
+    unpack<T, RAGGED>(x, count, d);
     unsigned bits = 0;
     if (a.drop.threshold) {
         bits = drop_bits(a.drop, key, static_cast<unsigned>(row), static_cast<unsigned>(unit));
@@ -329,7 +329,7 @@ __device__ __forceinline__ void store_grads(const NormBwdArgs& a, const DropKey&
     if constexpr (JOIN) {
         if (a.dh) {
             float d[kUnit];
-            unpack<S, RAGGED>(dh, count, a.C, d);
+            unpack<S, RAGGED>(dh, count, d);
 #pragma unroll
             for (int j = 0; j < kUnit; ++j) out[j] += d[j];
         }
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_bwd(NormBwdArg
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         count[i] = unit_count<RAGGED>(a.C, i * lanes + sub);
-        load_typed<RAGGED>(a.gamma, a.param_type, static_cast<long long>(i * lanes + sub) * kUnit, count[i], a.C, 1.f, ga[i]);
+        load_typed<RAGGED>(a.gamma, a.param_type, static_cast<long long>(i * lanes + sub) * kUnit, count[i], 1.f, ga[i]);
 #pragma unroll
         for (int j = 0; j < kUnit; ++j) dg[i][j] = db[i][j] = 0.f;
     }
@@ -380,10 +380,10 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_bwd(NormBwdArg
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int unit = i * lanes + sub;
-            h_next[i] = load_raw<H, RAGGED>(static_cast<const typename H::store*>(a.h) + at * a.h_ld + static_cast<long long>(unit) * kUnit, live, count[i], a.C);
-            g_next[i] = load_raw<T, RAGGED>(static_cast<const typename T::store*>(a.dy) + at * a.dy_ld + static_cast<long long>(unit) * kUnit, live, count[i], a.C);
-            if constexpr (SUM) x_next[i] = load_raw<T, RAGGED>(static_cast<const typename T::store*>(a.x) + at * a.x_ld + static_cast<long long>(unit) * kUnit, live, count[i], a.C);
-            if (JOIN && a.dh) d_next[i] = load_raw<S, RAGGED>(static_cast<const typename S::store*>(a.dh) + at * a.dh_ld + static_cast<long long>(unit) * kUnit, live, count[i], a.C);
+            h_next[i] = load_raw<H, RAGGED>(static_cast<const typename H::store*>(a.h) + at * a.h_ld + static_cast<long long>(unit) * kUnit, live, count[i]);
+            g_next[i] = load_raw<T, RAGGED>(static_cast<const typename T::store*>(a.dy) + at * a.dy_ld + static_cast<long long>(unit) * kUnit, live, count[i]);
+            if constexpr (SUM) x_next[i] = load_raw<T, RAGGED>(static_cast<const typename T::store*>(a.x) + at * a.x_ld + static_cast<long long>(unit) * kUnit, live, count[i]);
+            if (JOIN && a.dh) d_next[i] = load_raw<S, RAGGED>(static_cast<const typename S::store*>(a.dh) + at * a.dh_ld + static_cast<long long>(unit) * kUnit, live, count[i]);
         }
         mean_next = live ? a.mean[row] : 0.f;                                      // (a row that is none has xhat 0, whatever row 0 holds)
         rstd_next = live ? a.rstd[row] : 0.f;
@@ -401,9 +401,9 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void k_norm_bwd(NormBwdArg
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             dh[i] = d_next[i];
-            unpack<H, RAGGED>(h_next[i], count[i], a.C, xhat[i]);
+            unpack<H, RAGGED>(h_next[i], count[i], xhat[i]);
             if constexpr (SUM) bits[i] = sum_again<T, RAGGED>(a, key, at, i * lanes + sub, count[i], x_next[i], xhat[i]);
-            unpack<T, RAGGED>(g_next[i], count[i], a.C, gg[i]);
+            unpack<T, RAGGED>(g_next[i], count[i], gg[i]);
         }
         if (first + step < a.rows) fetch(first + step);
 #pragma unroll
@@ -497,15 +497,15 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormBwdArgs a) {
             for (int u = threadIdx.x; u < units; u += blockDim.x) {
                 const int count = unit_count<2>(a.C, u);
                 const long long c = static_cast<long long>(u) * kUnit;
-                load_unit<H, 2>(static_cast<const typename H::store*>(a.h) + row * a.h_ld + c, count, a.C, xhat);
+                load_unit<H, 2>(static_cast<const typename H::store*>(a.h) + row * a.h_ld + c, count, xhat);
                 unsigned bits = 0;
                 if constexpr (SUM) {
-                    const Raw<T> x = load_raw<T, 2>(static_cast<const typename T::store*>(a.x) + row * a.x_ld + c, true, count, a.C);
+                    const Raw<T> x = load_raw<T, 2>(static_cast<const typename T::store*>(a.x) + row * a.x_ld + c, true, count);
                     bits = sum_again<T, 2>(a, key, row, u, count, x, xhat);
                 }
-                load_unit<T, 2>(static_cast<const typename T::store*>(a.dy) + row * a.dy_ld + c, count, a.C, gg);
+                load_unit<T, 2>(static_cast<const typename T::store*>(a.dy) + row * a.dy_ld + c, count, gg);
                 float ga[kUnit];
-                load_typed<2>(a.gamma, a.param_type, c, count, a.C, 1.f, ga);
+                load_typed<2>(a.gamma, a.param_type, c, count, 1.f, ga);
 #pragma unroll
                 for (int j = 0; j < kUnit; ++j) {
                     xhat[j] = (xhat[j] - mean) * rstd;
@@ -520,7 +520,7 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormBwdArgs a) {
                     }
                 } else {
                     Raw<S> dh = {};
-                    if (JOIN && a.dh) dh = load_raw<S, 2>(static_cast<const typename S::store*>(a.dh) + row * a.dh_ld + c, true, count, a.C);
+                    if (JOIN && a.dh) dh = load_raw<S, 2>(static_cast<const typename S::store*>(a.dh) + row * a.dh_ld + c, true, count);
                     store_grads<T, S, JOIN, 2, SUM>(a, key, row, u, count, gg, xhat, dh, bits, rstd, m1, m2);
                 }
             }
@@ -541,12 +541,12 @@ __global__ __launch_bounds__(256) void k_norm_bwd_cols_long(NormBwdArgs a) {
     if constexpr (SUM)
         if (a.drop.threshold) key = drop_key(a.drop);
     for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
-        load_unit<H, 2>(static_cast<const typename H::store*>(a.h) + row * a.h_ld + c, count, a.C, h);
+        load_unit<H, 2>(static_cast<const typename H::store*>(a.h) + row * a.h_ld + c, count, h);
         if constexpr (SUM) {
-            const Raw<T> x = load_raw<T, 2>(static_cast<const typename T::store*>(a.x) + row * a.x_ld + c, true, count, a.C);
+            const Raw<T> x = load_raw<T, 2>(static_cast<const typename T::store*>(a.x) + row * a.x_ld + c, true, count);
             sum_again<T, 2>(a, key, row, unit, count, x, h);
         }
-        load_unit<T, 2>(static_cast<const typename T::store*>(a.dy) + row * a.dy_ld + c, count, a.C, g);
+        load_unit<T, 2>(static_cast<const typename T::store*>(a.dy) + row * a.dy_ld + c, count, g);
         const float mean = a.mean[row], rstd = a.rstd[row];
 #pragma unroll
         for (int j = 0; j < kUnit; ++j) {
@@ -599,7 +599,9 @@ inline int even_blocks(int64_t passes, int64_t most) {
 // columns: 44 us with 2, 48 with 8 for 480,000 rows), and every workgroup of the backward pass leaves a partial row (4096 bf16
 // columns, 8192 rows: 44 us with 1, 55 with 4).  Forward: 512 lanes with 32 bytes or 1024 with 16 (4096 bf16 columns: 36 us with
 // 1 workgroup, 24 with 4; 101 fp32, joined: 57 with 2, 60 with 4); half as many again for ragged 16-bit rows of one unit a lane, which
-// are bound by their arithmetic (501 bf16, joined: 58 with 6, 64 with 4, 63 with 8).  Backward, whose next row is on its
+// are bound by their arithmetic (30 million bf16 values, us with 4, 6, 8 workgroups, alone and joined: 9 columns 44 41 49, 95 81 92;
+// 35: 44 39 48, 99 86 94; 133: 48 40 46, 113 99 101; 301: 45 38 43, 105 94 97; 501: 31 27 32, 69 61 67; rows of a workgroup, 1101: 49 40 36,
+// 94 83 84; 2001: 32 27 29, 60 58 63; fewer than 4 are slower throughout).  Backward, whose next row is on its
 // way already: 16 KB of each tensor in flight where wavefronts hold the rows (bf16, 64 columns: 73 us with 1, 39 with 4, 44 with 8), 8 KB
 // where workgroups do.
 inline int norm_fwd_per_cu(const NormShape& s, int C, int unit_bytes) {

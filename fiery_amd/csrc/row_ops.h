@@ -123,7 +123,7 @@ __device__ __forceinline__ Raw<T> load_pieces(const typename T::store* p, int co
     return r;
 }
 template <typename T, int RAGGED>
-__device__ __forceinline__ Raw<T> load_raw(const typename T::store* p, bool live, int count, int C) {
+__device__ __forceinline__ Raw<T> load_raw(const typename T::store* p, bool live, int count) {
     if (RAGGED == 3) return load_pieces<T>(p, live ? count : 0);
     Raw<T> r = {};
     if (live && count > 0) {
@@ -134,7 +134,7 @@ __device__ __forceinline__ Raw<T> load_raw(const typename T::store* p, bool live
     return r;
 }
 template <typename T, int RAGGED>
-__device__ __forceinline__ void unpack(Raw<T> r, int count, int C, float (&v)[kUnit]) {
+__device__ __forceinline__ void unpack(Raw<T> r, int count, float (&v)[kUnit]) {
     constexpr int kWords = sizeof(typename T::store) * kUnit / 4;
     const unsigned off = (RAGGED == 1 || RAGGED == 2) && count > 0 ? kUnit - count : 0;
     if (RAGGED == 1 || (RAGGED == 2 && off)) {
@@ -158,8 +158,8 @@ __device__ __forceinline__ void unpack(Raw<T> r, int count, int C, float (&v)[kU
     }
 }
 template <typename T, int RAGGED>
-__device__ __forceinline__ void load_unit(const typename T::store* p, int count, int C, float (&v)[kUnit]) {
-    unpack<T, RAGGED>(load_raw<T, RAGGED>(p, true, count, C), count, C, v);
+__device__ __forceinline__ void load_unit(const typename T::store* p, int count, float (&v)[kUnit]) {
+    unpack<T, RAGGED>(load_raw<T, RAGGED>(p, true, count), count, v);
 }
 // (a store of less than a unit goes in pieces)
 template <typename T, int RAGGED>
@@ -183,16 +183,16 @@ __device__ __forceinline__ void store_unit(typename T::store* p, int count, cons
 
 // parameters, whose type is known at run time only: read once per lane, outside the loops
 template <int RAGGED>
-__device__ __forceinline__ void load_typed(const void* p, int type, long long c, int count, int C, float otherwise, float (&v)[kUnit]) {
+__device__ __forceinline__ void load_typed(const void* p, int type, long long c, int count, float otherwise, float (&v)[kUnit]) {
     if (!p) {
 #pragma unroll
         for (int j = 0; j < kUnit; ++j) v[j] = otherwise;
     } else if (type == FIERY_TYPE_F32) {
-        load_unit<F32, RAGGED>(static_cast<const float*>(p) + c, count, C, v);
+        load_unit<F32, RAGGED>(static_cast<const float*>(p) + c, count, v);
     } else if (type == FIERY_TYPE_BF16) {
-        load_unit<BF16, RAGGED>(static_cast<const unsigned short*>(p) + c, count, C, v);
+        load_unit<BF16, RAGGED>(static_cast<const unsigned short*>(p) + c, count, v);
     } else {
-        load_unit<F16, RAGGED>(static_cast<const unsigned short*>(p) + c, count, C, v);
+        load_unit<F16, RAGGED>(static_cast<const unsigned short*>(p) + c, count, v);
     }
 }
 __device__ __forceinline__ void store_typed(void* p, int type, long long i, float v) {
