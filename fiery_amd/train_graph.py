@@ -692,7 +692,7 @@ class TrainGraph:
         if again:
             if _capturing(x):
                 raise RuntimeError('dropout under saved-tensor hooks (activation checkpointing) cannot be captured into a graph')
-            call = int(torch.randint(1 << 62, (1,)))
+            call = int(torch.randint(1 << 62, (1,), device='cpu'))
             rng = rng.clone()
             rng[1:].zero_()
         elif torch._C._current_graph_task_id() != -1:
