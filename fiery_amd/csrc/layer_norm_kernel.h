@@ -10,7 +10,7 @@
 // eight columns (row_ops.h): a power-of-two group of up to 64 lanes of one wavefront (C <= 1024, no barrier), a workgroup (up
 // to 8192), or, past that, a workgroup that walks the row three times.
 // The mean itself is corrected by the mean of the distances from it, and the variance by that correction's square: the sum of a row's
-// values is rounded (1000 values of 12345.678 had a mean off by 0.0016, y by 0.5).  Where the correction is no small part of the
+// values is rounded (1000 values of 12345.678 had a mean off by 0.002, y by 0.5).  Where the correction is no small part of the
 // variance (values closer together than their sum's rounding: constant rows), the distances are taken once more.  It costs one value
 // more in the second exchange: 90,720 x 128 fp16 forward 11.2 us, 10.3 without; 8192 x 4096 bf16 27 and 26, joined 53 and 52.
 // The backward pass deals a lane the same columns for all its rows, so dgamma and dbeta grow in registers; every workgroup
@@ -24,9 +24,11 @@
 // against 65; 8192 x 4096 bf16: 90 - 95 against 73 - 80, both with the sum of the partial rows).
 //
 // Measured (one MI355X; a large copy reaches 5.35 TB/s): 480,000 x 64 fp32 forward 46 us = 5.4 TB/s, backward 69 + 5 us = 5.0 TB/s,
-// joined 94 and 120 + 5 us = 5.2 and 4.9 TB/s; 8192 x 4096 bf16 28 and 39 + 4 us = 4.7 TB/s, joined 53 and 63 + 5 us = 5.1 and 5.0 TB/s;
-// 90,720 x 128 fp16 forward 11 us = 4.1 TB/s.  Counter traffic is the operands' and the partial rows'.  240,000 x 35 bf16: 14 and 18 + 5 us
-// = 2.4 and 2.1 TB/s, bound by instructions (five of a group's eight lanes hold columns).
+// joined 95 and 120 + 5 us = 5.2 and 4.9 TB/s; 8192 x 4096 bf16 29 and 39 + 4 us = 4.7 TB/s, joined 52 and (SUM) 87 + 5 us = 5.1 and 4.4 TB/s,
+// beside an fp32 stream 72 and 102 + 5 us = 5.6 and 4.9 TB/s; 90,720 x 128 fp16 forward 11 - 12 us = 3.9 TB/s.  Counter traffic is the
+// operands' and the partial rows'.  240,000 x 35 bf16: 14 and 19 + 5 us = 2.4 and 2.1 TB/s, joined 30 and (SUM) 39 + 5 us, bound by
+// instructions: the layout puts five units on eight lanes.  3000 x 10,000 bf16 (three walks): 45 and 45 + 22 + 10 us = 2.7 and 1.2 TB/s,
+// joined 104 and (SUM) 127 + 32 + 10 us: the walks after the first come out of the caches.
 #pragma once
 #include "row_ops.h"
 
