@@ -450,3 +450,34 @@ def test_the_call_table_sees_the_row_operators(on, monkeypatch):  # noqa: F811
     monkeypatch.setattr(native, 'CALL_SINK', None)
     dx, = torch.autograd.grad(y, leaf, torch.ones_like(y))
     assert torch.equal(dx, torch.autograd.grad(row_ops.layer_norm(leaf, lib=on.lib), leaf, torch.ones_like(y))[0])
+
+
+@pytest.mark.gpu
+def test_a_captured_step_at_the_unrounded_sum(hip):
+    """keep='inputs' forward and backward in one hipGraph, rows of which some are constant (their squares are taken twice): every replay
+    equals the eager step of its numbers bit for bit, with eager work in between."""
+    for shape in ((60, 50, 64), (200, 2056), (30, 9000)):
+        x, r, w, b, dy, dh = [t.detach() for t in join_case(type('On', (), dict(device='cuda')), shape, BF16, F32)]
+        x[3], r[3] = 12.3, 4.1
+
+        def step(rng):
+            leaves = [t.detach().requires_grad_() for t in (x, r, w, b)]
+            y, h = row_ops.dropout_add_layer_norm(*leaves, 0.3, rng, keep='inputs')
+            grads = torch.autograd.grad((y, h), leaves, (dy, dh))
+            rng[1:].add_(1)
+            return [y.detach(), h.detach(), *grads]
+        rng, eager = row_ops.dropout_rng(8, 'cuda'), row_ops.dropout_rng(8, 'cuda')
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(rng)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(rng)
+        eager[1] += 1
+        for _ in range(3):
+            graph.replay()
+            want = step(eager)
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(out, want)) and torch.equal(rng, eager)
